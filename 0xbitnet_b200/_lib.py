@@ -58,6 +58,13 @@ SIGNATURES = {
                                        _P]),
     "obn_attention_decode_rope_at": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _F, _F, _P, _P,
                                           _SZ, _P]),
+    "obn_rope_kv_append_q8": (_I, [_P, _I, _I, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P, _P, _I,
+                                   _P]),
+    "obn_kv_read_q8": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P]),
+    "obn_attention_q8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "obn_attention_q8": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _F, _P, _P, _SZ,
+                              _P]),
+    "obn_logits_process": (_I, [_P, _I, _I, _P, _P, _P, _P]),
     "obn_add": (_I, [_P, _P, _SZ, _P, _P]),
     "obn_embed_f16": (_I, [_P, _I, _I, _P, _I, _P, _P]),
     "obn_rmsnorm_quantize": (_I, [_P, _P, _F, _I, _I, _P, _P, _P, _P]),
@@ -67,6 +74,16 @@ SIGNATURES = {
     "obn_bitlinear_export_i2s": (_I, [_P, _P, _P]),
     "obn_check_device_errors": (_I, []),
 }
+
+
+class LogitRulesStruct(ctypes.Structure):
+    """obn_logit_rules of include/obn.h."""
+
+    _fields_ = [("repetition", _P), ("frequency", _P), ("presence", _P),
+                ("history", _P), ("history_lens", _P), ("history_ld", ctypes.c_int64),
+                ("bias_ids", _P), ("bias_values", _P), ("bias_lens", _P),
+                ("bias_ld", ctypes.c_int64), ("mask", _P), ("mask_ld", ctypes.c_int64),
+                ("history_cap", ctypes.c_int32), ("bias_cap", ctypes.c_int32)]
 
 
 class ObnError(RuntimeError):

@@ -92,3 +92,149 @@ def attention_rope(qkv: torch.Tensor, cache: KVCache, H: int, pos: int,
                                           _ptr(out), _ptr(ws), ws.numel(), _stream(qkv.device)))
     cache.seq_len = max(cache.seq_len, pos + 1)
     return out
+
+
+# ---- KV cache in 8 bits -------------------------------------------------------------------
+
+Q8_BLOCK = 16  # positions that share a scale
+
+
+def _check_cuda(t, name: str, dtype, device=None) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.is_contiguous()):
+        raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+
+
+class KVCacheQ8:
+    """Caches of one layer in 8 bits: int8 codes k, v [B, S_max, Hkv, head_dim] and f32
+    power-of-two scales k_scale, v_scale [B, ceil(S_max / 16), Hkv]; the row at position p
+    stands for codes * scale of block p // 16. Half the bytes of KVCache."""
+
+    def __init__(self, B: int, S_max: int, Hkv: int, head_dim: int = 128, device=None):
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        codes = [torch.zeros((B, S_max, Hkv, head_dim), dtype=torch.int8, device=device)
+                 for _ in range(2)]
+        scales = [torch.zeros((B, -(-S_max // Q8_BLOCK), Hkv), dtype=torch.float32,
+                              device=device) for _ in range(2)]
+        self._init(codes[0], scales[0], codes[1], scales[1])
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor,
+             v_scale: torch.Tensor) -> "KVCacheQ8":
+        """A cache over existing buffers (not copied)."""
+        self = cls.__new__(cls)
+        for t, name in ((k, "k"), (v, "v")):
+            _check_cuda(t, name, torch.int8, k.device)
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _check_cuda(t, name, torch.float32, k.device)
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("k and v must be [B, S_max, Hkv, head_dim], of one shape")
+        want = (k.shape[0], -(-k.shape[1] // Q8_BLOCK), k.shape[2])
+        if tuple(k_scale.shape) != want or tuple(v_scale.shape) != want:
+            raise ValueError(f"k_scale and v_scale must be {want}")
+        self._init(k, k_scale, v, v_scale)
+        return self
+
+    def _init(self, k, k_scale, v, v_scale):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.B, self.S_max, self.Hkv, self.head_dim = k.shape
+        self.device = k.device
+        self.seq_len = 0
+
+    def read(self, first: int | torch.Tensor, count: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The values of rows first .. first + count - 1 of every sequence (an int, or an
+        int32 tensor [B] on the device) as f32 k, v [B, count, Hkv, head_dim]; rows outside
+        the cache are zero."""
+        k = torch.empty((self.B, count, self.Hkv, self.head_dim), dtype=torch.float32,
+                        device=self.device)
+        v = torch.empty_like(k)
+        host, dev = _host_or_dev(first, self, "first")
+        with _on(self.device):
+            check(lib().obn_kv_read_q8(
+                self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                self.v_scale.data_ptr(), self.B, self.Hkv, self.head_dim, self.S_max, host, dev,
+                count, k.data_ptr(), v.data_ptr(), _stream(self.device)))
+        return k, v
+
+
+def _on(device):
+    """The device as the current one for the launches below."""
+    return torch.cuda.device(device)
+
+
+def _host_or_dev(value, cache: KVCacheQ8, name: str) -> tuple[int, int | None]:
+    """(host value, None) of an int, (0, address) of an int32 tensor [B] on the device."""
+    if isinstance(value, torch.Tensor):
+        _check_cuda(value, name, torch.int32, cache.device)
+        if value.numel() != cache.B:
+            raise ValueError(f"{name} must hold one value for each of {cache.B} sequences")
+        return 0, value.data_ptr()
+    return int(value), None
+
+
+def _q8_rows(t, name: str, cache: KVCacheQ8, rows: int, cols: int) -> None:
+    _check_cuda(t, name, torch.float32, cache.device)
+    if t.numel() != rows * cols:
+        raise ValueError(f"{name} must be [{rows}, {cols}]")
+
+
+def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
+                      theta_base: float = 500000.0, q_out: torch.Tensor | None = None,
+                      pos: int | torch.Tensor | None = None) -> torch.Tensor:
+    """rope_kv_append into the 8-bit cache: qkv [B*n, (H + 2*Hkv) * d] f32 -> rotated q
+    [B*n, H*d]; token t of sequence b is stored at position pos + t (pos[b] + t for an int32
+    tensor [B] on the device; cache.seq_len by default). Tokens whose position is outside
+    the cache are not stored and get a zero q row when pos is a tensor, and are refused when
+    it is an int."""
+    B, Hkv, d = cache.B, cache.Hkv, cache.head_dim
+    _q8_rows(qkv, "qkv", cache, B * n, (H + 2 * Hkv) * d)
+    if q_out is None:
+        q_out = torch.empty((B * n, H * d), dtype=torch.float32, device=cache.device)
+    else:
+        _q8_rows(q_out, "q_out", cache, B * n, H * d)
+    host, dev = _host_or_dev(cache.seq_len if pos is None else pos, cache, "pos")
+    with _on(cache.device):
+        check(lib().obn_rope_kv_append_q8(
+            qkv.data_ptr(), B, n, H, Hkv, d, host, dev, theta_base, q_out.data_ptr(),
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), cache.S_max, _stream(cache.device)))
+    return q_out
+
+
+def attention_q8_workspace(cache: KVCacheQ8, H: int, n: int) -> torch.Tensor:
+    """A workspace for attention_q8 of n new tokens, at every length of the cache. One call
+    at a time may use it."""
+    need = int(lib().obn_attention_q8_workspace_bytes(cache.B, n, H, cache.Hkv, cache.head_dim,
+                                                      cache.S_max))
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=cache.device)
+
+
+def attention_q8(q: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
+                 seq_len: int | torch.Tensor, scale: float | None = None,
+                 out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                 max_len: int | None = None) -> torch.Tensor:
+    """Causal GQA attention of the n newest tokens over the 8-bit cache: q [B*n, H*d] -> out
+    [B*n, H*d]. The sequences hold seq_len positions each (an int), or seq_len[b] (an int32
+    tensor [B] on the device, at most max_len, by default the cache's S_max). Query t sees
+    keys [0, seq_len - n + t]; one that sees none gives a zero row."""
+    B, Hkv, d = cache.B, cache.Hkv, cache.head_dim
+    _q8_rows(q, "q", cache, B * n, H * d)
+    sc = 1.0 / float(np.sqrt(np.float32(d))) if scale is None else scale
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _q8_rows(out, "out", cache, B * n, H * d)
+    if workspace is None:
+        workspace = attention_q8_workspace(cache, H, n)
+    else:
+        _check_cuda(workspace, "workspace", torch.uint8, cache.device)
+    host, dev = _host_or_dev(seq_len, cache, "seq_len")
+    if dev is not None:
+        host = cache.S_max if max_len is None else max_len
+    with _on(cache.device):
+        check(lib().obn_attention_q8(
+            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), B, n, H, Hkv, d, cache.S_max, host, dev, sc,
+            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(cache.device)))
+    return out

@@ -16,6 +16,8 @@
 #include "layout.cuh"
 #include "lmhead.h"
 #include "attention.h"
+#include "kvq8.h"
+#include "logits.h"
 
 struct obn_bitlinear {
   int device = 0;
@@ -882,6 +884,151 @@ int obn_attention_decode_rope_at(const float* qkv, void* k_cache, void* v_cache,
   if (!pos_dev) return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
   return attention_rope_common(qkv, k_cache, v_cache, B, H, Hkv, head_dim, S_max, 0, pos_dev,
                                theta_base, scale, out, workspace, workspace_bytes, stream);
+}
+
+namespace {
+// What the entry points of the 8-bit cache check alike.
+int check_q8(const void* k_cache, const void* v_cache, const float* k_scale,
+             const float* v_scale, int B, int Hkv, int head_dim, int S_max) {
+  if (!k_cache || !v_cache || !k_scale || !v_scale)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (B <= 0 || Hkv <= 0 || S_max <= 0)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "need B, Hkv and S_max > 0 (got %d, %d, %d)", B, Hkv,
+                S_max);
+  if (head_dim != obn::kQ8HeadDim)
+    return fail(OBN_ERR_UNSUPPORTED, "head_dim must be %d (got %d)", obn::kQ8HeadDim, head_dim);
+  if (B > 65535 || Hkv > 65535 || S_max > (1 << 30))
+    return fail(OBN_ERR_UNSUPPORTED, "at most 65535 sequences and KV heads and 2^30 positions");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scale, 4) ||
+      !aligned(v_scale, 4))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "caches must be 16-byte, scales 4-byte aligned");
+  return OBN_OK;
+}
+
+int check_q8_heads(int B, int n, int H, int Hkv) {
+  if (n <= 0 || H <= 0) return fail(OBN_ERR_INVALID_ARGUMENT, "need n and H > 0 (got %d, %d)", n, H);
+  if (H % Hkv != 0 || H / Hkv > obn::kQ8MaxGroup)
+    return fail(OBN_ERR_UNSUPPORTED, "H must be 1 to %d times Hkv (got %d / %d)",
+                obn::kQ8MaxGroup, H, Hkv);
+  if (static_cast<long long>(B) * n * H > (1ll << 30))
+    return fail(OBN_ERR_UNSUPPORTED, "%d x %d tokens of %d heads are too many", B, n, H);
+  return OBN_OK;
+}
+}  // namespace
+
+int obn_rope_kv_append_q8(const float* qkv, int B, int n, int H, int Hkv, int head_dim, int pos,
+                          const int* pos_dev, float theta_base, float* q_out, void* k_cache,
+                          void* v_cache, float* k_scale, float* v_scale, int S_max, void* stream) {
+  clear_error();
+  if (!qkv || !q_out) return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (int rc = check_q8(k_cache, v_cache, k_scale, v_scale, B, Hkv, head_dim, S_max)) return rc;
+  if (int rc = check_q8_heads(B, n, H, Hkv)) return rc;
+  if (!pos_dev && (pos < 0 || static_cast<long long>(pos) + n > S_max))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "positions %d..%lld are not in the cache of %d", pos,
+                static_cast<long long>(pos) + n - 1, S_max);
+  if (!(theta_base > 0.0f))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "theta_base must be positive");
+  if (!aligned(qkv, 16) || !aligned(q_out, 16) || (pos_dev && !aligned(pos_dev, 4)))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "qkv and q_out must be 16-byte aligned");
+  const obn::Q8Cache c{static_cast<int8_t*>(k_cache), static_cast<int8_t*>(v_cache), k_scale,
+                       v_scale, B, S_max, Hkv};
+  cudaError_t e = obn::launch_rope_append_q8(qkv, c, n, H, pos, pos_dev, theta_base, q_out,
+                                             static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rope / 8-bit kv append launch");
+  return OBN_OK;
+}
+
+int obn_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale,
+                   const float* v_scale, int B, int Hkv, int head_dim, int S_max, int first,
+                   const int* first_dev, int count, float* k_out, float* v_out, void* stream) {
+  clear_error();
+  if (!k_out && !v_out) return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (int rc = check_q8(k_cache, v_cache, k_scale, v_scale, B, Hkv, head_dim, S_max)) return rc;
+  if (count <= 0) return fail(OBN_ERR_INVALID_ARGUMENT, "count must be positive (got %d)", count);
+  if (static_cast<long long>(B) * count * Hkv > (1ll << 33))
+    return fail(OBN_ERR_UNSUPPORTED, "%d x %d rows of %d heads are too many", B, count, Hkv);
+  if ((k_out && !aligned(k_out, 16)) || (v_out && !aligned(v_out, 16)) ||
+      (first_dev && !aligned(first_dev, 4)))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "k_out and v_out must be 16-byte aligned");
+  const obn::Q8Cache c{static_cast<int8_t*>(const_cast<void*>(k_cache)),
+                       static_cast<int8_t*>(const_cast<void*>(v_cache)),
+                       const_cast<float*>(k_scale), const_cast<float*>(v_scale), B, S_max, Hkv};
+  cudaError_t e = obn::launch_read_q8(c, first, first_dev, count, k_out, v_out,
+                                      static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "8-bit kv read launch");
+  return OBN_OK;
+}
+
+size_t obn_attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int head_dim, int S_max) {
+  if (B <= 0 || n <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || head_dim != obn::kQ8HeadDim ||
+      S_max <= 0)
+    return 0;
+  return obn::attention_q8_workspace_bytes(B, n, H, Hkv, S_max);
+}
+
+int obn_attention_q8(const float* q, const void* k_cache, const void* v_cache,
+                     const float* k_scale, const float* v_scale, int B, int n, int H, int Hkv,
+                     int head_dim, int S_max, int seq_len, const int* seq_lens_dev, float scale,
+                     float* out, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (!q || !out || !workspace) return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (int rc = check_q8(k_cache, v_cache, k_scale, v_scale, B, Hkv, head_dim, S_max)) return rc;
+  if (int rc = check_q8_heads(B, n, H, Hkv)) return rc;
+  if (seq_len < 0 || seq_len > S_max)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "need 0 <= seq_len <= S_max (got %d, %d)", seq_len,
+                S_max);
+  const size_t need = obn::attention_q8_workspace_bytes(B, n, H, Hkv, S_max);
+  if (workspace_bytes < need)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "workspace of %zu bytes is smaller than the %zu needed",
+                workspace_bytes, need);
+  if (!aligned(workspace, 256) || !aligned(q, 16) || !aligned(out, 16) ||
+      (seq_lens_dev && !aligned(seq_lens_dev, 4)))
+    return fail(OBN_ERR_INVALID_ARGUMENT,
+                "q and out must be 16-byte, workspace 256-byte aligned");
+  const obn::Q8Cache c{static_cast<int8_t*>(const_cast<void*>(k_cache)),
+                       static_cast<int8_t*>(const_cast<void*>(v_cache)),
+                       const_cast<float*>(k_scale), const_cast<float*>(v_scale), B, S_max, Hkv};
+  cudaError_t e = obn::launch_attention_q8(q, c, n, H, seq_len, seq_lens_dev, scale, out,
+                                           workspace, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "8-bit cache attention launch");
+  return OBN_OK;
+}
+
+int obn_logits_process(const float* logits, int rows, int vocab, const obn_logit_rules* rules,
+                       float* out, int32_t* token, void* stream) {
+  clear_error();
+  if (!logits || !rules || !out) return fail(OBN_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (rows <= 0 || vocab <= 0)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "need rows and vocab > 0 (got %d, %d)", rows, vocab);
+  if (rows > 65535 || vocab > (1 << 24))
+    return fail(OBN_ERR_UNSUPPORTED, "at most 65535 rows and 2^24 ids (got %d, %d)", rows, vocab);
+  if (rules->history && (rules->history_cap < 0 || rules->history_cap > 65535))
+    return fail(OBN_ERR_UNSUPPORTED, "history_cap must be in 0..65535 (got %d)",
+                rules->history_cap);
+  if (rules->bias_ids && (rules->bias_cap < 0 || rules->bias_cap > 1024))
+    return fail(OBN_ERR_UNSUPPORTED, "bias_cap must be in 0..1024 (got %d)", rules->bias_cap);
+  if (!rules->bias_ids != !rules->bias_values)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "bias_ids and bias_values go together");
+  const int64_t words = (static_cast<int64_t>(vocab) + 31) / 32;
+  if ((rules->history && rules->history_ld != 0 && rules->history_ld < rules->history_cap) ||
+      (rules->bias_ids && rules->bias_ld != 0 && rules->bias_ld < rules->bias_cap) ||
+      (rules->mask && rules->mask_ld != 0 && rules->mask_ld < words))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "a list's rows overlap: its ld is below its length");
+  for (const void* p : {static_cast<const void*>(logits), static_cast<const void*>(out),
+                        static_cast<const void*>(token), static_cast<const void*>(rules->mask),
+                        static_cast<const void*>(rules->repetition),
+                        static_cast<const void*>(rules->frequency),
+                        static_cast<const void*>(rules->presence),
+                        static_cast<const void*>(rules->history),
+                        static_cast<const void*>(rules->history_lens),
+                        static_cast<const void*>(rules->bias_ids),
+                        static_cast<const void*>(rules->bias_values),
+                        static_cast<const void*>(rules->bias_lens)})
+    if (!aligned(p, 4)) return fail(OBN_ERR_INVALID_ARGUMENT, "pointers must be 4-byte aligned");
+  cudaError_t e = obn::launch_logits_process(logits, rows, vocab, *rules, out, token,
+                                             static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "logit rules launch");
+  return OBN_OK;
 }
 
 int obn_add(const float* a, const float* b, size_t count, float* y, void* stream) {

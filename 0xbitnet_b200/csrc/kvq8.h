@@ -1,0 +1,48 @@
+// kvq8.h — the 8-bit KV cache (kvq8.cu): RoPE + quantizing append, read-back and attention.
+//
+// Cache of one layer: codes int8 [B][S_max][Hkv][128] for keys and for values, and one f32
+// scale for each (sequence, block of kQ8Block positions, KV head): [B][ceil(S_max / 16)][Hkv].
+// The row at position p stands for codes * scale of block p / 16. Scales are powers of two
+// (or 0 for a block of zeros, NaN for a block that took a non-finite value).
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+namespace obn {
+
+constexpr int kQ8HeadDim = 128;  // head_dim the kernels are built for
+constexpr int kQ8Block = 16;     // positions that share a scale
+constexpr int kQ8MaxGroup = 8;   // query heads per KV head
+
+struct Q8Cache {
+  int8_t* k;       // [B][S_max][Hkv][128]
+  int8_t* v;
+  float* k_scale;  // [B][ceil(S_max / 16)][Hkv]
+  float* v_scale;
+  int B, S_max, Hkv;
+};
+
+inline int q8_blocks(int S_max) { return (S_max + kQ8Block - 1) / kQ8Block; }
+
+// Rotates q and k of token t of sequence b at position pos + t (pos_dev[b] + t when pos_dev
+// is given), writes q_out [B*n, H*128] and stores k and v into the cache.
+cudaError_t launch_rope_append_q8(const float* qkv, const Q8Cache& c, int n, int H, int pos,
+                                  const int* pos_dev, float theta_base, float* q_out,
+                                  cudaStream_t s);
+
+// Rows [first, first + count) of every sequence (first_dev[b] when given) as f32
+// [B][count][Hkv][128]; rows outside the cache are zero. k_out / v_out may be null.
+cudaError_t launch_read_q8(const Q8Cache& c, int first, const int* first_dev, int count,
+                           float* k_out, float* v_out, cudaStream_t s);
+
+// Causal GQA attention of the n newest tokens; sequence b holds seq_len positions, or
+// min(max(lens_dev[b], 0), seq_len) when lens_dev is given.
+size_t attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int S_max);
+cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, int seq_len,
+                                const int* lens_dev, float scale, float* out, void* workspace,
+                                cudaStream_t s);
+
+}  // namespace obn

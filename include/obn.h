@@ -290,6 +290,96 @@ OBN_API int obn_attention_decode_rope_at(const float* qkv, void* k_cache, void* 
                                          float* out, void* workspace, size_t workspace_bytes,
                                          void* stream);
 
+/* ---- KV cache in 8 bits ------------------------------------------------------------ */
+/* No counterpart in the reference (its cache is f32). The cache of one layer holds int8
+ * codes k_cache / v_cache [B][S_max][Hkv][head_dim] (16-byte aligned) and f32 scales
+ * k_scale / v_scale [B][ceil(S_max / 16)][Hkv]: the row at position p is codes * scale of
+ * block p / 16 of its sequence and KV head. Scales are powers of two, 0 for a block of
+ * zeros, NaN for a block that took a NaN or an infinity (what reads it gives NaN). Start
+ * from zeroed buffers. Half the bytes of the binary16 cache of obn_rope_kv_append.
+ *
+ * obn_rope_kv_append with that cache: qkv [B*n, (H + 2*Hkv) * head_dim] f32; token t of
+ * sequence b sits at position pos + t, or pos_dev[b] + t when pos_dev (device, [B]) is not
+ * NULL. q and k are rotated by pos * theta_base^(-2i / head_dim) with angles in f64 (the
+ * binary16 append follows the shader's f32 angles, which drift at far positions). Writes
+ * q_out [B*n, H * head_dim] f32 and, for each touched block of 16 positions and KV head,
+ *   s = the smallest power of two (>= 2^-126) with |x| <= 127 s for every appended x, or
+ *       the block's scale if that is larger and the block has earlier rows;
+ *   appended rows: rint(x / s); rows of the block before them: rint(code * old s / s).
+ * A block's rows requantize only when its scale grows, which at least doubles it, so a held
+ * value is within s of the appended one (s / 2 if nothing larger came later). Rows of the
+ * block behind the appended ones keep their codes and lose their meaning: append in order.
+ * A token whose position is outside [0, S_max) is stored nowhere and gets a zero q row (left
+ * padding and idle sequences: a negative pos_dev[b]); without pos_dev, 0 <= pos and
+ * pos + n <= S_max are checked. Needs head_dim == 128, H a multiple of Hkv and
+ * H / Hkv <= 8; qkv and q_out 16-byte aligned. */
+OBN_API int obn_rope_kv_append_q8(const float* qkv, int B, int n, int H, int Hkv, int head_dim,
+                                  int pos, const int* pos_dev, float theta_base, float* q_out,
+                                  void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                  int S_max, void* stream);
+
+/* Rows [first, first + count) of every sequence, or from first_dev[b] when first_dev (device,
+ * [B]) is not NULL, as f32 [B][count][Hkv][head_dim] into k_out and / or v_out (16-byte
+ * aligned; one of them may be NULL). Rows outside [0, S_max) are zero. */
+OBN_API int obn_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale,
+                           const float* v_scale, int B, int Hkv, int head_dim, int S_max,
+                           int first, const int* first_dev, int count, float* k_out,
+                           float* v_out, void* stream);
+
+/* Scratch bytes of obn_attention_q8 for these sizes and every length up to S_max. */
+OBN_API size_t obn_attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int head_dim,
+                                                int S_max);
+
+/* obn_attention_decode over that cache: causal GQA attention of the n newest tokens of B
+ * sequences, q [B*n, H * head_dim] f32 -> out [B*n, H * head_dim] f32. Sequence b holds
+ * L = seq_len positions, or L = seq_lens_dev[b] brought into [0, seq_len] when seq_lens_dev
+ * (device, [B]) is not NULL: seq_len is then their bound (S_max if nothing better is known;
+ * the closer the bound, the better the split). Its query t attends to keys
+ * [0, L - n + t]; a query without keys (an empty sequence, left padding) gives a zero row.
+ * Sums are exact integers or f32, so results are within f32 rounding of the cache's values.
+ * Needs head_dim == 128, H a multiple of Hkv, H / Hkv <= 8 and 0 <= seq_len <= S_max; q and
+ * out 16-byte, workspace 256-byte aligned, not used by other work in flight. */
+OBN_API int obn_attention_q8(const float* q, const void* k_cache, const void* v_cache,
+                             const float* k_scale, const float* v_scale, int B, int n, int H,
+                             int Hkv, int head_dim, int S_max, int seq_len,
+                             const int* seq_lens_dev, float scale, float* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* ---- logit rules -------------------------------------------------------------------- */
+/* What a server lays on each row of logits before a token is picked. Device pointers, each
+ * NULL when the rule is not used. A list [rows][cap] has its rows `ld` elements apart (ld 0:
+ * one list for all rows); its length in row r is lens[r] brought into [0, cap], or cap when
+ * lens is NULL. Ids outside [0, vocab) are ignored. */
+typedef struct obn_logit_rules {
+  const float* repetition;     /* [rows], > 0: once for each occurrence in the history a
+                                  positive logit is divided and another one multiplied by it
+                                  (sampling.rs:14-27); default 1 */
+  const float* frequency;      /* [rows]: subtracted once for each occurrence; default 0 */
+  const float* presence;       /* [rows]: subtracted if the id occurs at all; default 0 */
+  const int32_t* history;      /* token ids, history_cap <= 65535 */
+  const int32_t* history_lens;
+  int64_t history_ld;
+  const int32_t* bias_ids;     /* ids and the biases added to them (the same id twice: both),
+                                  bias_cap <= 1024 */
+  const float* bias_values;
+  const int32_t* bias_lens;
+  int64_t bias_ld;
+  const uint32_t* mask;        /* ceil(vocab / 32) words a row: bit v % 32 of word v / 32 set =
+                                  token v allowed, else its logit becomes -inf */
+  int64_t mask_ld;
+  int32_t history_cap;
+  int32_t bias_cap;
+} obn_logit_rules;
+
+/* out[r, v] = the logits [rows, vocab] under the rules, in the order above: repetition,
+ * frequency and presence, biases, mask; a changed value is computed in f64 and rounded once,
+ * the others pass unchanged. out may be logits itself. token (nullable, [rows]) takes each
+ * row's greedy choice: the largest out[r, v], the lowest v among equals, NaN never; -1 when
+ * nothing is above -inf. A single occurrence gives the bits of the sampler's own penalty. */
+OBN_API int obn_logits_process(const float* logits, int rows, int vocab,
+                               const obn_logit_rules* rules, float* out, int32_t* token,
+                               void* stream);
+
 /* ---- decoder glue ------------------------------------------------------------- */
 /* Residual add (elementwise.wgsl op 0, TransformerBlock::forward's dispatch_add,
  * transformer.rs:63,69): y[i] = a[i] + b[i] for i < count (f32; y may alias a or b). */

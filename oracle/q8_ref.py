@@ -1,0 +1,116 @@
+"""CPU restatements in 64 bits of the 8-bit KV cache and the logit rules — TEST INFRASTRUCTURE
+ONLY. Plain numpy from the formulas in include/obn.h, one block, row or id at a time."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+
+BLOCK = 16
+MIN_EXP = -126
+
+
+def rope(x, pos, base):
+    """x [heads, d] of one token at position pos, rotated pair by pair."""
+    d = x.shape[-1]
+    i = np.arange(d // 2, dtype=np.float64)
+    ang = pos * np.power(np.float64(base), -2.0 * i / d)
+    c, s = np.cos(ang), np.sin(ang)
+    y = np.empty(x.shape, np.float64)
+    x = x.astype(np.float64)
+    y[..., 0::2] = x[..., 0::2] * c - x[..., 1::2] * s
+    y[..., 1::2] = x[..., 0::2] * s + x[..., 1::2] * c
+    return y
+
+
+def need_scale(x):
+    """The smallest power of two s >= 2^-126 with |x| <= 127 s; 0 for zeros, NaN for others."""
+    if not np.all(np.isfinite(x)):
+        return math.nan
+    a = float(np.max(np.abs(x))) if x.size else 0.0
+    if a == 0.0:
+        return 0.0
+    e = MIN_EXP
+    while a > 127.0 * 2.0 ** e:
+        e += 1
+    return 2.0 ** e
+
+
+def append(codes, scales, rows, pos):
+    """Appends rows [n, Hkv, d] (f64) at positions pos ... to one sequence's codes
+    [S_max, Hkv, d] (int) and scales [blocks, Hkv], in place. Returns the unrounded codes of
+    the stored rows [S_max, Hkv, d] (NaN elsewhere) for a test of borderline roundings."""
+    S_max = codes.shape[0]
+    raw = np.full(codes.shape, np.nan)
+    n = rows.shape[0]
+    lo, hi = max(pos, 0), min(pos + n, S_max)
+    for blk in range(lo // BLOCK, -(-hi // BLOCK) if hi > lo else 0):
+        a, b = max(lo, blk * BLOCK), min(hi, blk * BLOCK + BLOCK)
+        for h in range(codes.shape[1]):
+            new = rows[a - pos:b - pos, h]
+            had = a > blk * BLOCK
+            was = float(scales[blk, h]) if had else 0.0
+            need = need_scale(new)
+            now = math.nan if math.isnan(was) or math.isnan(need) else max(was, need)
+            scales[blk, h] = now
+            if not now > 0.0:
+                codes[a:b, h] = 0
+                continue
+            old = codes[blk * BLOCK:a, h].astype(np.float64)
+            codes[blk * BLOCK:a, h] = np.rint(old * (was / now))
+            raw[a:b, h] = new / now
+            codes[a:b, h] = np.rint(raw[a:b, h])
+    return raw
+
+
+def values(codes, scales):
+    """codes [S, Hkv, d] with scales [blocks, Hkv] -> f64 values."""
+    wide = np.repeat(scales.astype(np.float64), BLOCK, axis=0)[:codes.shape[0]]
+    return codes.astype(np.float64) * wide[:, :, None]
+
+
+def attention(q, k, v, L, scale):
+    """q [n, H, d] of the n newest of L positions over values k, v [>= L, Hkv, d] -> (out
+    [n, H, d], bound [n, H]): bound is how far an f32 evaluation may be off (see below).
+
+    With u = 2^-24: a score is a sum of products q_i k_i whose magnitudes add up to A; in at
+    most 24 accumulation steps of at most 2 u each, of q split to 2^-22, it is off by at most
+    48 u A, so a weight is off by that share (and 4 u of the exponential), which moves the
+    output by at most twice that times max |v|; sums over up to L keys in f32, a truncating
+    step of 2 u per 16 keys and half, add L / 2 u max |v|."""
+    n, H, d = q.shape
+    G = H // k.shape[1]
+    out = np.zeros((n, H, d))
+    bound = np.zeros((n, H))
+    for t in range(n):
+        lim = min(L, L - n + t + 1)
+        if lim <= 0:
+            continue
+        for h in range(H):
+            K, V = k[:lim, h // G], v[:lim, h // G]
+            s = K @ q[t, h].astype(np.float64) * scale
+            p = np.exp(s - s.max())
+            out[t, h] = p @ V / p.sum()
+            A = np.max(np.abs(K) @ np.abs(q[t, h].astype(np.float64))) * abs(scale)
+            bound[t, h] = np.abs(V).max() * 2.0 ** -24 * (2 * 48 * A + 64 + lim / 2)
+    return out, bound
+
+
+def logits(x, repetition=1.0, frequency=0.0, presence=0.0, history=(), bias=(), mask=None):
+    """One row x [V]: history a list of ids, bias a list of (id, value), mask [V] bool."""
+    y = x.astype(np.float64)
+    V = y.size
+    count = {}
+    for i in history:
+        if 0 <= i < V:
+            count[i] = count.get(i, 0) + 1
+    for i, c in count.items():
+        f = float(repetition) ** c
+        y[i] = y[i] / f if y[i] > 0 else y[i] * f
+        y[i] -= c * float(frequency) + float(presence)
+    for i, b in bias:
+        if 0 <= i < V:
+            y[i] += float(b)
+    if mask is not None:
+        y[~mask] = -np.inf
+    return y
