@@ -1,4 +1,5 @@
-// kvq8.cu — the KV cache held in 8 bits, sm_100a: append, read-back and attention.
+// kvq8.cu — the KV cache held in 8 bits, sm_100a: append and read-back
+// (attention over it: kvq8_attn.cu).
 //
 // Format. A row x of 128 values (a rotated key or a value) at position p is held as int8
 // codes c with x ~ c * s, where s = 2^e is shared by the 16 positions of a block and one KV
@@ -8,8 +9,6 @@
 // With powers of two s / s' is exact and a scale at least doubles when it grows, so the
 // roundings of a row add up to at most s/2 (1 + 1/2 + 1/4 + ...) <= s of its last scale.
 #include "kvq8.h"
-
-#include <cfloat>
 
 #include "obn_common.cuh"
 
@@ -171,94 +170,6 @@ __global__ __launch_bounds__(256) void k_read_q8(Q8Cache c, int first, const int
   }
 }
 
-// Attention of one query row and one KV head's group: 128 threads over chunks of 128 keys,
-// thread = key for the scores, thread = dimension for the weighted sum of V.
-__global__ __launch_bounds__(D) void k_attn_q8_row(const float* __restrict__ q, Q8Cache c, int n,
-                                                   int H, int seq_len,
-                                                   const int* __restrict__ lens_dev, float scale,
-                                                   float* __restrict__ out) {
-  __shared__ float s_q[kQ8MaxGroup][D], s_p[kQ8MaxGroup][D], s_red[kQ8MaxGroup][4], s_v[D];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int tid = threadIdx.x, G = H / c.Hkv, kvh = blockIdx.y;
-  const size_t r = blockIdx.x;
-  const int t = static_cast<int>(r % n);
-  const size_t b = r / n;
-  const int len = lens_dev ? min(max(lens_dev[b], 0), seq_len) : seq_len;
-  const int limit = min(len, len - n + t + 1);
-  const size_t nblk = (c.S_max + kQ8Block - 1) / kQ8Block;
-  for (int g = 0; g < G; ++g) s_q[g][tid] = q[(r * H + kvh * G + g) * D + tid];
-  float m[kQ8MaxGroup], l[kQ8MaxGroup], o[kQ8MaxGroup];
-  for (int g = 0; g < kQ8MaxGroup; ++g) {
-    m[g] = -INFINITY;
-    l[g] = o[g] = 0.0f;
-  }
-  for (int k0 = 0; k0 < limit; k0 += D) {
-    __syncthreads();
-    const int key = k0 + tid;
-    const bool seen = key < limit;
-    float sc[kQ8MaxGroup] = {};
-    if (seen) {
-      const char4* row = reinterpret_cast<const char4*>(
-          c.k + ((b * c.S_max + key) * c.Hkv + kvh) * D);
-      const size_t si = (b * nblk + key / kQ8Block) * c.Hkv + kvh;
-      for (int d = 0; d < D / 4; ++d) {
-        const char4 w = row[d];
-        for (int g = 0; g < kQ8MaxGroup; ++g)
-          if (g < G)
-            sc[g] += s_q[g][4 * d] * w.x + s_q[g][4 * d + 1] * w.y + s_q[g][4 * d + 2] * w.z +
-                     s_q[g][4 * d + 3] * w.w;
-      }
-      s_v[tid] = c.v_scale[si];
-      for (int g = 0; g < kQ8MaxGroup; ++g) sc[g] *= c.k_scale[si] * scale;
-    }
-    for (int g = 0; g < G; ++g) {
-      float w = seen ? sc[g] : -INFINITY;
-      for (int x = 16; x; x >>= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, x));
-      if (tid % 32 == 0) s_red[g][tid / 32] = w;
-    }
-    __syncthreads();
-    for (int g = 0; g < kQ8MaxGroup; ++g)
-      if (g < G) {
-        const float mn = fmaxf(fmaxf(fmaxf(s_red[g][0], s_red[g][1]), fmaxf(s_red[g][2], s_red[g][3])), m[g]);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float corr = expf(m[g] - base);
-        m[g] = mn;
-        l[g] *= corr;
-        o[g] *= corr;
-        s_p[g][tid] = seen ? expf(sc[g] - base) : 0.0f;
-      }
-    __syncthreads();
-    const int cnt = min(D, limit - k0);
-    for (int k = 0; k < cnt; ++k) {
-      const float v = c.v[((b * c.S_max + k0 + k) * c.Hkv + kvh) * D + tid] * s_v[k];
-      for (int g = 0; g < kQ8MaxGroup; ++g)
-        if (g < G) {
-          l[g] += s_p[g][k];
-          o[g] += s_p[g][k] * v;
-        }
-    }
-  }
-  for (int g = 0; g < kQ8MaxGroup; ++g)
-    if (g < G) out[(r * H + kvh * G + g) * D + tid] = limit > 0 ? o[g] / l[g] : 0.0f;
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
-
 }  // namespace
 
 cudaError_t launch_rope_append_q8(const float* qkv, const Q8Cache& c, int n, int H, int pos,
@@ -275,18 +186,6 @@ cudaError_t launch_read_q8(const Q8Cache& c, int first, const int* first_dev, in
   const size_t total = static_cast<size_t>(c.B) * count * c.Hkv * (D / 4);
   return launch_pdl(k_read_q8, dim3(static_cast<unsigned>((total + 255) / 256)), 256, 0, s, c, first,
                     first_dev, count, k_out, v_out, total);
-}
-
-size_t attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int S_max) {
-  (void)B, (void)n, (void)H, (void)Hkv, (void)S_max;
-  return 256;
-}
-
-cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, int seq_len,
-                                const int* lens_dev, float scale, float* out, void*,
-                                cudaStream_t s) {
-  return launch_pdl(k_attn_q8_row, dim3(static_cast<unsigned>(c.B) * n, c.Hkv), D, 0, s, q, c, n, H,
-                    seq_len, lens_dev, scale, out);
 }
 
 }  // namespace obn
