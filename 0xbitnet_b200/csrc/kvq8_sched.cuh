@@ -44,73 +44,34 @@ OBN_DEVINL int q8_units(const Q8Sched& s, int item) {
 OBN_DEVINL int q8_ctas(const Q8Sched& s, long long total) {
   return static_cast<int>(min(static_cast<long long>(s.ctas), total));
 }
+// The first unit of CTA c, and the CTA that holds unit x.
 OBN_DEVINL long long q8_begin(long long total, int ctas, int c) { return c * total / ctas; }
-// The CTA that holds unit x.
 OBN_DEVINL int q8_owner(long long total, int ctas, long long x) {
   return static_cast<int>(((x + 1) * ctas - 1) / total);
-}
-
-// For all THREADS threads of the CTA: the total of units, and with `before` items given the
-// units in front of item `before` (sh: THREADS + 1 shared words).
-template <int THREADS>
-OBN_DEVINL long long q8_total(const Q8Sched& s, int before, long long* in_front, long long* sh) {
-  const int items = s.B * s.tiles, tid = threadIdx.x;
-  if (!s.lens && s.tiles == 1) {
-    const long long u = q8_units(s, 0);
-    *in_front = u * before * s.Hkv;
-    return u * items * s.Hkv;
-  }
-  long long all = 0, front = 0;
-  for (int i = tid; i < items; i += THREADS) {
-    const int u = q8_units(s, i);
-    all += u;
-    if (i < before) front += u;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, d);
-    front += __shfl_xor_sync(0xffffffffu, front, d);
-  }
-  constexpr int W = THREADS / 32;
-  if (tid % 32 == 0) {
-    sh[tid / 32] = all;
-    sh[W + tid / 32] = front;
-  }
-  __syncthreads();
-  all = front = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    all += sh[w];
-    front += sh[W + w];
-  }
-  __syncthreads();
-  *in_front = front * s.Hkv;
-  return all * s.Hkv;
 }
 
 // A place in the row of units.
 struct Q8Cursor {
   int item, kvh, unit, units;  // units: those of the item
+  int b, tile, len;            // the item's sequence, its tile and the sequence's positions
 };
+OBN_DEVINL void q8_enter(const Q8Sched& s, Q8Cursor& c) {
+  c.b = c.item / s.tiles;
+  c.tile = c.item - c.b * s.tiles;
+  c.len = q8_len(s, c.b);
+}
 
-// The item, KV head and unit of unit `x` < total: each thread adds up a run of items, a scan
-// finds the run, its thread walks it. sh: THREADS + 4 shared words.
+// Adds up every item's units over the THREADS threads of the CTA, a run of items for each:
+// *front the units of the items before this thread's run, i0 .. i1 - 1 (times Hkv). Returns
+// the total. sh: THREADS / 32 shared words.
 template <int THREADS>
-OBN_DEVINL Q8Cursor q8_find(const Q8Sched& s, long long x, long long* sh) {
+OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* front, long long* sh) {
   const int items = s.B * s.tiles, tid = threadIdx.x;
-  Q8Cursor c;
-  if (!s.lens && s.tiles == 1) {
-    c.units = q8_units(s, 0);
-    const long long pair = x / c.units;
-    c.item = static_cast<int>(pair / s.Hkv);
-    c.kvh = static_cast<int>(pair % s.Hkv);
-    c.unit = static_cast<int>(x % c.units);
-    return c;
-  }
   const int per = (items + THREADS - 1) / THREADS;
-  const int i0 = min(tid * per, items), i1 = min(i0 + per, items);
+  *i0 = min(tid * per, items);
+  *i1 = min(*i0 + per, items);
   long long sum = 0;
-  for (int i = i0; i < i1; ++i) sum += q8_units(s, i);
+  for (int i = *i0; i < *i1; ++i) sum += q8_units(s, i);
   sum *= s.Hkv;
   long long incl = sum;
 #pragma unroll
@@ -120,28 +81,91 @@ OBN_DEVINL Q8Cursor q8_find(const Q8Sched& s, long long x, long long* sh) {
   }
   if (tid % 32 == 31) sh[tid / 32] = incl;
   __syncthreads();
-  for (int w = 0; w < tid / 32; ++w) incl += sh[w];
-  long long at = incl - sum;
-  if (x >= at && x < incl) {
-    int i = i0;
-    for (;; ++i) {
-      const long long u = static_cast<long long>(q8_units(s, i)) * s.Hkv;
-      if (x < at + u) break;
-      at += u;
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w == tid / 32) incl += total;
+    total += sh[w];
+  }
+  *front = incl - sum;
+  return total;
+}
+
+// This CTA's share: *mine units from the returned place on, 0 for a CTA without one. For all
+// threads; sh: THREADS / 32 + 8 shared words.
+template <int THREADS>
+OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, int* mine, long long* sh) {
+  Q8Cursor c = {};
+  if (!s.lens && s.tiles == 1) {  // all items alike
+    c.units = q8_units(s, 0);
+    const long long total = static_cast<long long>(c.units) * s.B * s.Hkv;
+    const int ctas = q8_ctas(s, total);
+    *mine = 0;
+    if (static_cast<int>(blockIdx.x) >= ctas) return c;
+    const long long x = q8_begin(total, ctas, blockIdx.x);
+    *mine = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+    const long long pair = x / c.units;
+    c.item = static_cast<int>(pair / s.Hkv);
+    c.kvh = static_cast<int>(pair - static_cast<long long>(c.item) * s.Hkv);
+    c.unit = static_cast<int>(x - pair * c.units);
+    q8_enter(s, c);
+    return c;
+  }
+  int i0, i1;
+  long long at;
+  const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
+  const int ctas = q8_ctas(s, total);
+  *mine = 0;
+  if (static_cast<int>(blockIdx.x) >= ctas) return c;
+  const long long x = q8_begin(total, ctas, blockIdx.x);
+  *mine = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+  if (x >= at) {  // the thread whose run holds unit x walks it
+    for (int i = i0; i < i1; ++i) {
+      const int u = q8_units(s, i);
+      const long long end = at + static_cast<long long>(u) * s.Hkv;
+      if (x < end) {
+        long long* o = sh + THREADS / 32;
+        o[0] = i;
+        o[1] = (x - at) / u;
+        o[2] = (x - at) % u;
+        o[3] = u;
+        o[4] = q8_len(s, i / s.tiles);
+        break;
+      }
+      at = end;
     }
-    const int u = q8_units(s, i);
-    sh[THREADS] = i;
-    sh[THREADS + 1] = (x - at) / u;
-    sh[THREADS + 2] = (x - at) % u;
-    sh[THREADS + 3] = u;
   }
   __syncthreads();
-  c.item = static_cast<int>(sh[THREADS]);
-  c.kvh = static_cast<int>(sh[THREADS + 1]);
-  c.unit = static_cast<int>(sh[THREADS + 2]);
-  c.units = static_cast<int>(sh[THREADS + 3]);
-  __syncthreads();
+  const long long* o = sh + THREADS / 32;
+  c.item = static_cast<int>(o[0]);
+  c.kvh = static_cast<int>(o[1]);
+  c.unit = static_cast<int>(o[2]);
+  c.units = static_cast<int>(o[3]);
+  c.len = static_cast<int>(o[4]);
+  c.b = c.item / s.tiles;
+  c.tile = c.item - c.b * s.tiles;
   return c;
+}
+
+// Where the parts of the pairs of item `item` are, for k_q8_join: the total, and in *front the
+// units before the item. For all threads; sh: THREADS / 32 + 1 shared words.
+template <int THREADS>
+OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, long long* sh) {
+  if (!s.lens && s.tiles == 1) {
+    const long long u = static_cast<long long>(q8_units(s, 0)) * s.Hkv;
+    *front = u * item;
+    return u * s.B;
+  }
+  int i0, i1;
+  long long at;
+  const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
+  if (i0 <= item && item < i1) {
+    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_units(s, i)) * s.Hkv;
+    sh[THREADS / 32] = at;
+  }
+  __syncthreads();
+  *front = sh[THREADS / 32];
+  return total;
 }
 
 // The next unit (the caller stops at the end of its share, so there is one).
@@ -155,6 +179,7 @@ OBN_DEVINL void q8_next(const Q8Sched& s, Q8Cursor& c) {
     if (++c.item >= items) return;
     c.units = q8_units(s, c.item);
   } while (c.units == 0);
+  q8_enter(s, c);
 }
 
 // Workspace of a pass of `rows` rows per tile: for each of 2 C slots the sums [rows][128],
