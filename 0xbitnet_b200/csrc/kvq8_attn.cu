@@ -140,14 +140,13 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   // the lengths may come from the kernel before; the join may read them once all are here
   pdl_wait();
   pdl_launch_dependents();
-  int mine;
-  Q8Cursor cur = q8_share<32 * (kWarps + 1)>(sc, &mine, sm.sh);
-  if (mine == 0) return;
+  Q8Cursor cur = q8_share<32 * (kWarps + 1)>(sc, sm.sh);
+  if (cur.left == 0) return;
   __syncthreads();
   const int H = sc.G * sc.Hkv, rows_seq = sc.n * sc.G;
 
   if (warp == kWarps) {  // producer
-    for (int it = 0; it < mine; ++it) {
+    for (int it = 0; cur.left > 0; ++it) {
       const int st = it % ST;
       if (it >= ST && !__all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (it / ST - 1) & 1))) return;
       const int k0 = cur.unit * kUnitKeys, left = cur.len - k0;
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
                        smem_u32(&sm.full[st]))
                    : "memory");
-      if (it + 1 < mine) q8_next(sc, cur);
+      q8_next(sc, cur);
     }
     return;
   }
@@ -258,7 +257,8 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
 
   fetch_q();
   bool fresh = true;
-  for (int it = 0; it < mine; ++it) {
+  int it = 0;
+  for (; cur.left > 0; ++it) {
     const int stage = it % ST;
     if (fresh) {  // a new pair
       fresh = false;
@@ -401,18 +401,13 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.empty[stage]);
 
-    const bool pair_ends = cur.unit + 1 == cur.units;
-    if (!pair_ends && it + 1 < mine) {
-      ++cur.unit;
-      continue;
-    }
+    const Q8Cursor done = cur;
+    q8_next(sc, cur);
+    const bool pair_ends = done.unit + 1 == done.units;
+    if (!pair_ends && cur.left > 0) continue;
     // merge the slices, write the pair or its part
     const bool whole = pair_ends && u_first == 0;
-    const Q8Cursor done = cur;
-    if (it + 1 < mine) {
-      q8_next(sc, cur);
-      fetch_q();
-    }
+    if (cur.left > 0) fetch_q();
     flush(M, Vr);
 #pragma unroll
     for (int d = 4; d <= 16; d <<= 1) l += shx(l, d);
@@ -472,71 +467,93 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     fresh = true;
   }
   if (dead)  // a copy may still be on its way into this CTA's shared memory
-    for (int i = 0; i < min(ST, mine); ++i) mbar_wait(&sm.full[i], ((mine - 1 - i) / ST) & 1);
+    for (int i = 0; i < min(ST, it); ++i) mbar_wait(&sm.full[i], ((it - 1 - i) / ST) & 1);
 }
 
 // Joins the parts of the pairs that span CTAs, and zeroes the pairs without keys. One CTA per
-// pair and row: four warps take every fourth part, a lane four dims. Where the parts are is
-// worked out while the pass before still runs.
-__global__ __launch_bounds__(128) void k_q8_join(Q8Sched sc, const float* __restrict__ ws_,
-                                                 float* __restrict__ out) {
-  __shared__ long long sh[4 + 1];
-  __shared__ float s_m[4], s_l[4];
-  __shared__ float4 s_o[4][32];
-  float* ws = const_cast<float*>(ws_);
+// pair and row; first the parts' maxima and totals, a lane a part, then their sums, a warp a
+// part at a time. Where the parts are is worked out while the pass before still runs.
+constexpr int kJoinWarps = 8;
+
+__global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, float* __restrict__ ws,
+                                                             float* __restrict__ out) {
+  __shared__ long long sh[kJoinWarps + 1];
+  __shared__ float s_w[kQ8MaxCtas];  // the parts' weights
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ float4 s_o[kJoinWarps][32];
   const int row = blockIdx.x % sc.tile_rows, kvh = blockIdx.y;
   const int item = blockIdx.x / sc.tile_rows;
   const int b = item / sc.tiles, tile = item - b * sc.tiles;
   const int r = tile * sc.tile_rows + row;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int t = r / sc.G, g = r - t * sc.G;
-  float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D;
   const int units = q8_units(sc, item);
   long long front;
-  const long long total = q8_locate<128>(sc, item, &front, sh);
-  const long long x0 = front + static_cast<long long>(kvh) * units;
-  const int ctas = q8_ctas(sc, total);
-  const int c0 = units ? q8_owner(total, ctas, x0) : 0;
-  const int c1 = units ? q8_owner(total, ctas, x0 + units - 1) : 0;
+  const long long total = q8_locate<32 * kJoinWarps>(sc, item, &front, sh);
+  int c0 = 0, c1 = 0;
+  if (units) {
+    const long long x0 = front + static_cast<long long>(kvh) * (units + 1) + 1;  // unit 0
+    const int ctas = q8_ctas(sc, total);
+    c0 = q8_owner(total, ctas, x0);
+    c1 = q8_owner(total, ctas, x0 + units - 1);
+  }
   pdl_wait();
   pdl_launch_dependents();
   if (r >= sc.n * sc.G) return;
+  const int t = r / sc.G, g = r - t * sc.G;
+  float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D;
   if (units == 0) {
     if (warp == 0) *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     return;
   }
   if (c0 == c1) return;  // written by its CTA
-  float m = -INFINITY, l = 0.0f;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    const int slot = 2 * c + (c == c0 ? 1 : 0);
-    const float* ml = q8_part_ml(ws, sc.tile_rows, slot);
-    const float pm = ml[row], pl = ml[sc.tile_rows + row];
-    const float4 x = *reinterpret_cast<const float4*>(q8_part_o(ws, sc.tile_rows, slot) + row * D + 4 * lane);
-    const float mn = fmaxf(m, pm);
-    const float e0 = m == mn ? 1.0f : ex2(m - mn), e1 = pm == mn ? 1.0f : ex2(pm - mn);
-    l = l * e0 + pl * e1;
-    y = make_float4(y.x * e0 + x.x * e1, y.y * e0 + x.y * e1, y.z * e0 + x.z * e1,
-                    y.w * e0 + x.w * e1);
-    m = mn;
+  const int parts = c1 - c0 + 1;
+  auto slot = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
+  constexpr int kPer = (kQ8MaxCtas + 32 * kJoinWarps - 1) / (32 * kJoinWarps);
+  float pm[kPer], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = tid + j * 32 * kJoinWarps;
+    pm[j] = i < parts ? q8_part_ml(ws, sc.tile_rows, slot(i))[row] : -INFINITY;
+    m = fmaxf(m, pm[j]);
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, shx(m, d));
+  if (lane == 0) s_m[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, s_m[w]);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = tid + j * 32 * kJoinWarps;
+    if (i < parts) {
+      // a part of NaN scores only has -inf here and its NaN in the total
+      const float e = pm[j] == m ? 1.0f : ex2(pm[j] - m);
+      s_w[i] = e;
+      l = fmaf(q8_part_ml(ws, sc.tile_rows, slot(i))[sc.tile_rows + row], e, l);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += shx(l, d);
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int i = warp; i < parts; i += kJoinWarps) {
+    const float4 x = *reinterpret_cast<const float4*>(
+        q8_part_o(ws, sc.tile_rows, slot(i)) + row * D + 4 * lane);
+    const float e = s_w[i];
+    y = make_float4(fmaf(x.x, e, y.x), fmaf(x.y, e, y.y), fmaf(x.z, e, y.z), fmaf(x.w, e, y.w));
   }
   s_o[warp][lane] = y;
   __syncthreads();
   if (warp) return;
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
   l = 0.0f;
   y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float e = s_m[w] == m ? 1.0f : ex2(s_m[w] - m);
+  for (int w = 0; w < kJoinWarps; ++w) {
     const float4 x = s_o[w][lane];
-    l += s_l[w] * e;
-    y = make_float4(y.x + x.x * e, y.y + x.y * e, y.z + x.z * e, y.w + x.w * e);
+    l += s_l[w];
+    y = make_float4(y.x + x.x, y.y + x.y, y.z + x.z, y.w + x.w);
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
@@ -568,13 +585,14 @@ cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale
   CUtensorMap mk, mv;
   if (!q8_map(&mk, c.k, c, kSlice) || !q8_map(&mv, c.v, c, kSlice)) return cudaErrorNotSupported;
   const long long bound = static_cast<long long>(sc.B) * sc.tiles * sc.Hkv *
-                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys);
+                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys + 1);
   const long long fit = std::min(num_sms_cached() * CTAS, kQ8MaxCtas);
   sc.ctas = static_cast<int>(std::max<long long>(std::min(bound, fit), 1));
   e = launch_pdl(&k_attn_q8_few<MT, KW, ST, CTAS>, dim3(sc.ctas), 32 * (MT * KW + 1), smem, s, mk, mv,
                  q, c.k_scale, c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, ws);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k_q8_join, dim3(sc.B * sc.tiles * sc.tile_rows, sc.Hkv), 128, 0, s, sc, ws, out);
+  return launch_pdl(k_q8_join, dim3(sc.B * sc.tiles * sc.tile_rows, sc.Hkv),
+                    32 * kJoinWarps, 0, s, sc, ws, out);
 }
 
 }  // namespace

@@ -2,10 +2,12 @@
 //
 // The query rows of a sequence and KV head (t * G + g for token t and group head g) are cut
 // into tiles of `tile_rows`; an item is a (sequence, tile), a pair an item with a KV head,
-// and a unit kUnitKeys keys of a pair. All units of all pairs in a row, T of them, are dealt
-// out evenly: CTA c of C <= T takes units [c T / C, (c + 1) T / C). So sequences of any mix of
-// lengths and causal tiles of any depth keep every CTA equally busy, and one long sequence
-// is split as finely as many short ones. A pair that lies inside one CTA is written
+// and a unit kUnitKeys keys of a pair. Every pair with keys is a start, which costs about as
+// much as a unit (64 sequences of up to 4095: without it the CTAs with 8 short pairs took 41
+// us, those with one 29), and then its units. All places of all pairs in a row, T of them, are
+// dealt out evenly: CTA c of C <= T takes places [c T / C, (c + 1) T / C). So sequences of any
+// mix of lengths and causal tiles of any depth keep every CTA equally busy, and one long
+// sequence is split as finely as many short ones. A pair that lies inside one CTA is written
 // out by it; the parts of a pair that spans CTAs go to the workspace and are joined by
 // k_q8_join. A CTA holds at most two parts: one that continues a pair (slot 2c) and one that
 // begins a pair and does not end it (slot 2c + 1).
@@ -40,20 +42,28 @@ OBN_DEVINL int q8_units(const Q8Sched& s, int item) {
   const int last = min((tile + 1) * s.tile_rows, s.n * s.G) - 1;
   return (max(q8_limit(s, q8_len(s, b), last), 0) + kUnitKeys - 1) / kUnitKeys;
 }
-// CTAs that take part: every one of them has a unit, and so a part where a pair spans it.
+// Places of a pair of `units` units.
+OBN_DEVINL int q8_places(int units) { return units + (units > 0 ? 1 : 0); }
+// CTAs that take part: every one of them has a place.
 OBN_DEVINL int q8_ctas(const Q8Sched& s, long long total) {
   return static_cast<int>(min(static_cast<long long>(s.ctas), total));
 }
-// The first unit of CTA c, and the CTA that holds unit x.
-OBN_DEVINL long long q8_begin(long long total, int ctas, int c) { return c * total / ctas; }
+// The first place of CTA c, and the CTA that holds place x.
+OBN_DEVINL long long q8_begin(long long total, int ctas, int c) {
+  if (total * ctas <= 0x7FFFFFFFll) return static_cast<int>(c * static_cast<int>(total)) / ctas;
+  return c * total / ctas;
+}
 OBN_DEVINL int q8_owner(long long total, int ctas, long long x) {
+  if (total * ctas <= 0x7FFFFFFFll)
+    return (static_cast<int>(x + 1) * ctas - 1) / static_cast<int>(total);
   return static_cast<int>(((x + 1) * ctas - 1) / total);
 }
 
-// A place in the row of units.
+// A unit on the way through a CTA's share.
 struct Q8Cursor {
   int item, kvh, unit, units;  // units: those of the item
   int b, tile, len;            // the item's sequence, its tile and the sequence's positions
+  int left;                    // places of the share from this unit on, 0: the share is done
 };
 OBN_DEVINL void q8_enter(const Q8Sched& s, Q8Cursor& c) {
   c.b = c.item / s.tiles;
@@ -61,8 +71,8 @@ OBN_DEVINL void q8_enter(const Q8Sched& s, Q8Cursor& c) {
   c.len = q8_len(s, c.b);
 }
 
-// Adds up every item's units over the THREADS threads of the CTA, a run of items for each:
-// *front the units of the items before this thread's run, i0 .. i1 - 1 (times Hkv). Returns
+// Adds up every item's places over the THREADS threads of the CTA, a run of items for each:
+// *front the places of the items before this thread's run, i0 .. i1 - 1 (times Hkv). Returns
 // the total. sh: THREADS / 32 shared words.
 template <int THREADS>
 OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* front, long long* sh) {
@@ -71,7 +81,7 @@ OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* fron
   *i0 = min(tid * per, items);
   *i1 = min(*i0 + per, items);
   long long sum = 0;
-  for (int i = *i0; i < *i1; ++i) sum += q8_units(s, i);
+  for (int i = *i0; i < *i1; ++i) sum += q8_places(q8_units(s, i));
   sum *= s.Hkv;
   long long incl = sum;
 #pragma unroll
@@ -91,68 +101,81 @@ OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* fron
   return total;
 }
 
-// This CTA's share: *mine units from the returned place on, 0 for a CTA without one. For all
-// threads; sh: THREADS / 32 + 8 shared words.
+// The first unit of this CTA's share (left 0: it has none). For all threads; sh: THREADS / 32
+// + 8 shared words.
 template <int THREADS>
-OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, int* mine, long long* sh) {
+OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
   Q8Cursor c = {};
+  int place;
   if (!s.lens && s.tiles == 1) {  // all items alike
     c.units = q8_units(s, 0);
-    const long long total = static_cast<long long>(c.units) * s.B * s.Hkv;
+    const int each = q8_places(c.units);
+    const long long total = static_cast<long long>(each) * s.B * s.Hkv;
     const int ctas = q8_ctas(s, total);
-    *mine = 0;
     if (static_cast<int>(blockIdx.x) >= ctas) return c;
     const long long x = q8_begin(total, ctas, blockIdx.x);
-    *mine = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
-    const long long pair = x / c.units;
-    c.item = static_cast<int>(pair / s.Hkv);
-    c.kvh = static_cast<int>(pair - static_cast<long long>(c.item) * s.Hkv);
-    c.unit = static_cast<int>(x - pair * c.units);
+    c.left = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+    long long pair;
+    if (total <= 0x7FFFFFFFll)
+      pair = static_cast<int>(x) / each;
+    else
+      pair = x / each;
+    c.item = static_cast<int>(pair) / s.Hkv;
+    c.kvh = static_cast<int>(pair) - c.item * s.Hkv;
+    place = static_cast<int>(x - pair * each);
     q8_enter(s, c);
-    return c;
-  }
-  int i0, i1;
-  long long at;
-  const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
-  const int ctas = q8_ctas(s, total);
-  *mine = 0;
-  if (static_cast<int>(blockIdx.x) >= ctas) return c;
-  const long long x = q8_begin(total, ctas, blockIdx.x);
-  *mine = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
-  if (x >= at) {  // the thread whose run holds unit x walks it
-    for (int i = i0; i < i1; ++i) {
-      const int u = q8_units(s, i);
-      const long long end = at + static_cast<long long>(u) * s.Hkv;
-      if (x < end) {
-        long long* o = sh + THREADS / 32;
-        o[0] = i;
-        o[1] = (x - at) / u;
-        o[2] = (x - at) % u;
-        o[3] = u;
-        o[4] = q8_len(s, i / s.tiles);
-        break;
+  } else {
+    int i0, i1;
+    long long at;
+    const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
+    const int ctas = q8_ctas(s, total);
+    if (static_cast<int>(blockIdx.x) >= ctas) return c;
+    const long long x = q8_begin(total, ctas, blockIdx.x);
+    c.left = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+    long long* o = sh + THREADS / 32;
+    if (x >= at) {  // the thread whose run holds place x walks it
+      for (int i = i0; i < i1; ++i) {
+        const int u = q8_units(s, i), each = q8_places(u);
+        const long long end = at + static_cast<long long>(each) * s.Hkv;
+        if (x < end) {
+          // a pair's places times Hkv fit 32 bits: at most 2^23 + 1 units times 65535
+          const unsigned long long in = static_cast<unsigned long long>(x - at);
+          const int kvh = in <= 0x7FFFFFFFull ? static_cast<int>(in) / each
+                                              : static_cast<int>(in / each);
+          o[0] = i;
+          o[1] = kvh;
+          o[2] = static_cast<long long>(in) - static_cast<long long>(kvh) * each;
+          o[3] = u;
+          o[4] = q8_len(s, i / s.tiles);
+          break;
+        }
+        at = end;
       }
-      at = end;
     }
+    __syncthreads();
+    c.item = static_cast<int>(o[0]);
+    c.kvh = static_cast<int>(o[1]);
+    place = static_cast<int>(o[2]);
+    c.units = static_cast<int>(o[3]);
+    c.len = static_cast<int>(o[4]);
+    c.b = c.item / s.tiles;
+    c.tile = c.item - c.b * s.tiles;
   }
-  __syncthreads();
-  const long long* o = sh + THREADS / 32;
-  c.item = static_cast<int>(o[0]);
-  c.kvh = static_cast<int>(o[1]);
-  c.unit = static_cast<int>(o[2]);
-  c.units = static_cast<int>(o[3]);
-  c.len = static_cast<int>(o[4]);
-  c.b = c.item / s.tiles;
-  c.tile = c.item - c.b * s.tiles;
+  if (place == 0) {  // a start
+    --c.left;
+    c.unit = 0;
+  } else {
+    c.unit = place - 1;
+  }
   return c;
 }
 
 // Where the parts of the pairs of item `item` are, for k_q8_join: the total, and in *front the
-// units before the item. For all threads; sh: THREADS / 32 + 1 shared words.
+// places before the item. For all threads; sh: THREADS / 32 + 1 shared words.
 template <int THREADS>
 OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, long long* sh) {
   if (!s.lens && s.tiles == 1) {
-    const long long u = static_cast<long long>(q8_units(s, 0)) * s.Hkv;
+    const long long u = static_cast<long long>(q8_places(q8_units(s, 0))) * s.Hkv;
     *front = u * item;
     return u * s.B;
   }
@@ -160,7 +183,7 @@ OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, lon
   long long at;
   const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
   if (i0 <= item && item < i1) {
-    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_units(s, i)) * s.Hkv;
+    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_places(q8_units(s, i))) * s.Hkv;
     sh[THREADS / 32] = at;
   }
   __syncthreads();
@@ -168,15 +191,16 @@ OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, lon
   return total;
 }
 
-// The next unit (the caller stops at the end of its share, so there is one).
+// Steps to the share's next unit; left becomes 0 at its end.
 OBN_DEVINL void q8_next(const Q8Sched& s, Q8Cursor& c) {
+  if (--c.left <= 0) return;
   if (++c.unit < c.units) return;
+  if (--c.left == 0) return;  // the next pair's start
   c.unit = 0;
   if (++c.kvh < s.Hkv) return;
   c.kvh = 0;
-  const int items = s.B * s.tiles;
   do {
-    if (++c.item >= items) return;
+    ++c.item;  // an item with units follows: the share has places left
     c.units = q8_units(s, c.item);
   } while (c.units == 0);
   q8_enter(s, c);
