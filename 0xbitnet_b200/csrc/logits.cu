@@ -5,17 +5,20 @@
 //   n > 0:  x > 0 ? x / rep^n : x * rep^n, then - (freq * n + pres)
 //   + the biases listed for v;  -inf where the mask's bit is 0;  token = argmax, lowest v
 //
-// The pass reads and writes 4 bytes a logit and should wait for nothing else. A cluster of
-// CTAs takes a row; each CTA copies its slice of it to shared memory and meanwhile counts the
-// occurrences of the slice's ids, by shared-memory atomics on whole numbers (16 bits an id),
-// so every order of arrival gives the same counts; every CTA of a row scans the whole
-// history, which lies in L2. In a second scan the first thread to claim an id (a bit in shared
-// memory) rewrites its logit there: the f64 work is spread over the threads as the history is, not as
-// the ids lie (histories crowd in a few slices: 123 us for 64 rows of 128256 with 4096 ids
-// when the threads that stream the logits did it in passing). Biases are compacted in list
-// order; the first entry of an id owns it and adds up the others in that order. A rewritten
-// logit is rounded once. Then the slice streams out, with the mask and the row's maximum, which
-// goes through shuffles, shared memory and the first CTA of the cluster.
+// The pass reads and writes 4 bytes a logit and should wait for nothing else. A row is cut
+// into slices of 8192 ids, which a cluster of CTAs (one to sixteen, as many as fit on the GPU at
+// once) takes in turn; a CTA has the next slice's logits on the way (one bulk copy) while it works
+// on one in shared memory, and the lists, read once, in registers:
+//   1. count the occurrences of the slice's ids (16 bits an id, shared-memory atomics on
+//      whole numbers: any order gives the same counts); an atomic that finds a zero puts
+//      the id on the slice's list of distinct ids
+//   2. the list's logits are rewritten in place, in f64, rounded once; an id with a bias is left
+//      to the first of its bias entries, which has the sum of all of them in list order
+//   3. the slice streams out, with the mask and the row's maximum
+// With the list the f64 work falls on full warps. Histories crowd in a few slices and are
+// sparse in the others: 64 rows of 128256 with 4096 ids took 123 us when the threads that stream
+// the logits rewrote them in passing, 38 us when the threads that count an id rewrote it,
+// 58 us with the history spread over the cluster and remote counters.
 #include "logits.h"
 
 #include <cmath>
@@ -24,60 +27,121 @@
 #include "obn_common.cuh"
 
 namespace obn {
+
+int num_sms_cached();  // kernels.cu
+
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kQuads = 8;                           // float4 per thread
-constexpr int kSliceIds = 4 * kQuads * kThreads;    // 16384
-constexpr int kMaxCluster = 8;
-constexpr int kMaxBias = 1024;
+constexpr int kQuads = 4;                         // float4 of a slice per thread
+constexpr int kSliceIds = 4 * kQuads * kThreads;  // 8192
+constexpr int kMaxCluster = 16;
+constexpr int kMaxBias = 1024, kBiasPer = kMaxBias / kThreads;
+constexpr int kHistRegs = 8;    // history entries of a thread in registers
 
 struct LogitSmem {
-  float x[kSliceIds];
-  uint32_t count[kSliceIds / 2];  // 16 bits an id
-  uint32_t taken[kSliceIds / 32];  // ids whose logit has an owner
-  int hit_id[kMaxBias];
-  float hit_value[kMaxBias];
-  int warp_hits[kThreads / 32];
+  float x[2][kSliceIds];
+  uint16_t count[kSliceIds];
+  uint16_t found[kSliceIds];  // distinct ids of the history in the slice
+  uint32_t founds;
+  uint32_t biased[kSliceIds / 32];  // ids with a bias, and with several
+  uint32_t twice[kSliceIds / 32];
+  int bias_id[kMaxBias];
+  float bias_value[kMaxBias];
   uint32_t best_key[kThreads / 32];
   uint32_t best_at[kThreads / 32];
   uint2 cluster_best[kMaxCluster];  // of the cluster's CTAs, in the first one
-  uint64_t full;
+  uint64_t full[2];
 };
 
 // base^n for n >= 1 in f64.
 OBN_DEVINL double ipow(double base, unsigned n) {
+  if (n == 1) return base;
   double r = 1.0;
   for (; n; n >>= 1, base *= base)
     if (n & 1) r *= base;
   return r;
 }
 
-// Order-preserving key of a float above -inf (0 stands for none; -0 counts as +0).
+constexpr int kNowhere = 0x7FFFFFFF;  // position of an id outside the row
+
+// Order-preserving key of a float that is no NaN (-0 counts as +0).
 OBN_DEVINL uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u << 1) == 0) return 0x80000000u;
+  const uint32_t u = __float_as_uint(x + 0.0f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ __launch_bounds__(kThreads) void k_logits(const float* __restrict__ logits, int V,
-                                                     obn_logit_rules u, int cluster,
-                                                     float* out, int32_t* __restrict__ token) {
+// Ids count from the 16-byte boundary at or before the row's start: position p = v + mis.
+__global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int V,
+                                                        obn_logit_rules u, float* out,
+                                                        int32_t* __restrict__ token) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   LogitSmem& sm = *reinterpret_cast<LogitSmem*>(smem_raw);
   pdl_launch_dependents();
-  pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x;
+  const int rank = blockIdx.x, cluster = gridDim.x;
   const size_t r = blockIdx.y;
+  if (tid == 0) {
+    mbar_init(&sm.full[0], 1);
+    mbar_init(&sm.full[1], 1);
+    fence_mbar_init();
+  }
+  for (int i = tid; i < kSliceIds / 8; i += kThreads)
+    reinterpret_cast<uint4*>(sm.count)[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int i = tid; i < kSliceIds / 32; i += kThreads) sm.biased[i] = sm.twice[i] = 0;
+  if (tid == 0) sm.founds = 0;
+  __syncthreads();
+  // waited for at the end: no store to a CTA that has not started
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  pdl_wait();
   const float* x_row = logits + r * V;
   float* y_row = out + r * V;
-  // Quad q holds ids 4 q - mis .. + 3: aligned 16 bytes of the row, whose ends may be cut.
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x_row) >> 2) & 3);
   const bool vec_out = (reinterpret_cast<uintptr_t>(y_row) & 15) == (reinterpret_cast<uintptr_t>(x_row) & 15);
-  const int quads = (V + mis + 3) / 4;
-  const int per = min((quads + cluster - 1) / cluster, kQuads * kThreads);  // quads of a slice
-  const uint32_t* mask = u.mask ? u.mask + r * u.mask_ld : nullptr;
+  const int end = V + mis;  // positions of the row: [mis, end)
+  const int step = cluster * kSliceIds;
+  bool dead = false;  // a copy did not come in time: no more of them
+
+  // Quads [q_head, q_end) of the slice at p0 lie in the row; one before them and one behind may
+  // be cut by the row's ends.
+  auto q_head = [&](int p0) { return p0 < mis ? 1 : 0; };
+  auto q_end = [&](int p0) {
+    const int cnt = min(kSliceIds, end - p0);
+    return max(cnt / 4, q_head(p0));
+  };
+  // The whole quads of the slice at p0 by one bulk copy, the cut ones at the row's ends by their
+  // elements (threads 0 to 7). Returns whether there is a copy to wait for.
+  auto request = [&](int p0, int buf) {
+    const int cnt = min(kSliceIds, end - p0), nq = (cnt + 3) / 4;
+    const int head = q_head(p0), whole = q_end(p0) - head;
+    if (tid == 0 && whole > 0 && !dead) {
+      fence_proxy_async_smem();  // threads read and wrote the buffer before
+      mbar_arrive_expect_tx(&sm.full[buf], whole * 16);
+      bulk_g2s(&sm.x[buf][4 * head], x_row + (p0 + 4 * head - mis), whole * 16, &sm.full[buf]);
+    }
+    if (tid < 8) {
+      const int i = 4 * (tid < 4 ? 0 : nq - 1) + (tid & 3), p = p0 + i;
+      if ((tid < 4 ? head : q_end(p0) < nq) && p >= mis && p < end) sm.x[buf][i] = x_row[p - mis];
+    }
+    return whole > 0;
+  };
+  const int p_first = rank * kSliceIds;
+  bool copied = p_first < end ? request(p_first, 0) : false;
+
+  // The lists, requested before their lengths are known.
+  const int32_t* h = u.history + r * u.history_ld;
+  int hid[kHistRegs], bid[kBiasPer];
+  float bval[kBiasPer];
+#pragma unroll
+  for (int i = 0; i < kHistRegs; ++i)
+    hid[i] = u.history && tid + i * kThreads < u.history_cap ? __ldg(h + tid + i * kThreads) : -1;
+#pragma unroll
+  for (int i = 0; i < kBiasPer; ++i) {
+    const int j = tid + i * kThreads;
+    const bool in = u.bias_ids && j < u.bias_cap;
+    bid[i] = in ? __ldg(u.bias_ids + r * u.bias_ld + j) : -1;
+    bval[i] = in ? __ldg(u.bias_values + r * u.bias_ld + j) : 0.0f;
+  }
   const int hist = !u.history ? 0 : u.history_lens ? min(max(u.history_lens[r], 0), u.history_cap)
                                                    : u.history_cap;
   const int nbias = !u.bias_ids ? 0 : u.bias_lens ? min(max(u.bias_lens[r], 0), u.bias_cap)
@@ -86,14 +150,20 @@ __global__ __launch_bounds__(kThreads) void k_logits(const float* __restrict__ l
   const double freq = u.frequency ? u.frequency[r] : 0.0f;
   const double pres = u.presence ? u.presence[r] : 0.0f;
   const double inv_rep = 1.0 / rep;
-  uint32_t best = 0, best_at = 0, phase = 0;
-  bool dead = false;  // a copy did not come in time: no more of them
-  if (tid == 0) {
-    mbar_init(&sm.full, 1);
-    fence_mbar_init();
+  // From here on the lists hold positions.
+  auto position = [&](int id) { return static_cast<unsigned>(id) < static_cast<unsigned>(V) ? id + mis : kNowhere; };
+#pragma unroll
+  for (int i = 0; i < kHistRegs; ++i)
+    hid[i] = tid + i * kThreads < hist ? position(hid[i]) : kNowhere;
+#pragma unroll
+  for (int i = 0; i < kBiasPer; ++i) {
+    const int j = tid + i * kThreads;
+    bid[i] = j < nbias ? position(bid[i]) : kNowhere;
+    if (nbias) {
+      sm.bias_id[j] = bid[i];
+      sm.bias_value[j] = bval[i];
+    }
   }
-  __syncthreads();
-
   // The logit of an id with n occurrences. 1 / rep in f64 serves for the division: quotients
   // of two f32 lie at least 2^-49 (relative) from the middle between two f32, the product is
   // off by 2^-52, so a single occurrence gives the correctly rounded quotient.
@@ -102,133 +172,159 @@ __global__ __launch_bounds__(kThreads) void k_logits(const float* __restrict__ l
     return x;
   };
 
-  for (int q0 = rank * per; q0 < quads; q0 += cluster * per) {
-    const int nq = min(per, quads - q0);
-    const int v0 = 4 * q0 - mis;  // the first id (may be below 0)
-    // 1. request the slice: whole quads by one bulk copy, cut ones by their elements
-    const int head = v0 < 0 ? 1 : 0, tail = v0 + 4 * nq > V && nq > head ? 1 : 0;
-    const int whole = nq - head - tail;
-    if (tid == 0 && whole > 0 && !dead) {
-      fence_proxy_async_smem();  // the slice before was read and written by threads
-      mbar_arrive_expect_tx(&sm.full, whole * 16);
-      bulk_g2s(&sm.x[4 * head], x_row + v0 + 4 * head, whole * 16, &sm.full);
-    }
-    if (tid < 8) {
-      const int q = tid < 4 ? 0 : nq - 1, i = 4 * q + (tid & 3), v = v0 + i;
-      if ((tid < 4 ? head : tail) && v >= 0 && v < V) sm.x[i] = x_row[v];
-    }
-    uint32_t allow[kQuads];
+  const uint32_t* mask = u.mask ? u.mask + r * u.mask_ld : nullptr;
+  float best = -INFINITY;
+  int best_at = 0;
+  uint32_t phase = 0;
+  int buf = 0;
+  for (int p0 = p_first; p0 < end; p0 += step, buf ^= 1) {
+    const int cnt = min(kSliceIds, end - p0), nq = (cnt + 3) / 4;
+    const bool wait = copied;
+    if (p0 + step < end) copied = request(p0 + step, buf ^ 1);
+    // mask words of the thread's quads, used when they have come
+    uint32_t m_lo[kQuads], m_hi[kQuads];
+    if (mask) {
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const int q = tid + k * kThreads, v = v0 + 4 * q;
-      allow[k] = 15u;
-      if (mask && q < nq) {
-        const int lo = max(v, 0) >> 5, hi = min(v + 3, V - 1) >> 5;
-        const uint32_t a = __ldg(mask + lo), b = hi != lo ? __ldg(mask + hi) : a;
-        allow[k] = v < 0 ? a << -v : __funnelshift_r(a, b, v & 31);
+      for (int k = 0; k < kQuads; ++k) {
+        const int q = tid + k * kThreads, v = p0 + 4 * q - mis;
+        const int lo = max(v, 0) >> 5, hi = mis ? min(v + 3, V - 1) >> 5 : lo;
+        m_lo[k] = q < nq ? __ldg(mask + lo) : 0;
+        m_hi[k] = hi != lo && q < nq ? __ldg(mask + hi) : 0;
       }
     }
-    // 2. occurrences and biases of the slice's ids
-    const int32_t* h = u.history + r * u.history_ld;
-    auto local = [&](int id) {  // index in the slice, or -1
-      const unsigned at = static_cast<unsigned>(id - v0);
-      return id >= 0 && id < V && at < static_cast<unsigned>(4 * nq) ? static_cast<int>(at) : -1;
+    auto allowed = [&](int k, int v) {  // bits 0 to 3: of ids v to v + 3
+      if (!mask) return 15u;
+      return v < 0 ? m_lo[k] << -v : __funnelshift_r(m_lo[k], m_hi[k], v & 31);
     };
+    auto in = [&](int at) { return static_cast<unsigned>(at) < static_cast<unsigned>(cnt); };
+    // 1. occurrences, distinct ids, biased ids
     if (hist) {
-      for (int i = tid; i < (nq + 1) / 2; i += kThreads)
-        reinterpret_cast<uint4*>(sm.count)[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    if (hist || nbias) {
-      for (int i = tid; i < (4 * nq + 31) / 32; i += kThreads) sm.taken[i] = 0;
-      __syncthreads();
-    }
-    for (int i = tid; i < hist; i += kThreads) {
-      const int at = local(__ldg(h + i));
-      if (at >= 0) atomicAdd(&sm.count[at >> 1], 1u << (16 * (at & 1)));
-    }
-    int hits = 0;
-    for (int j0 = 0; j0 < nbias; j0 += kThreads) {
-      const int j = j0 + tid;
-      const int id = j < nbias ? __ldg(u.bias_ids + r * u.bias_ld + j) : -1;
-      const int at = local(id);
-      const uint32_t votes = __ballot_sync(0xffffffffu, at >= 0);
-      if (lane == 0) sm.warp_hits[warp] = __popc(votes);
-      __syncthreads();
-      int before = hits;
+      auto occurs = [&](int at) {
+        const int sh = 16 * (at & 1);
+        const uint32_t was = atomicAdd(reinterpret_cast<uint32_t*>(sm.count) + (at >> 1), 1u << sh);
+        if (((was >> sh) & 0xFFFFu) == 0)
+          sm.found[atomicAdd(&sm.founds, 1u)] = static_cast<uint16_t>(at);
+      };
 #pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) {
-        const int n = sm.warp_hits[w];
-        if (w < warp) before += n;
-        hits += n;
+      for (int i = 0; i < kHistRegs; ++i)
+        if (in(hid[i] - p0)) occurs(hid[i] - p0);
+      for (int j = tid + kHistRegs * kThreads; j < hist; j += kThreads) {
+        const int at = position(__ldg(h + j)) - p0;
+        if (in(at)) occurs(at);
       }
-      if (at >= 0) {
-        const int place = before + __popc(votes & ((1u << lane) - 1u));
-        sm.hit_id[place] = at;
-        sm.hit_value[place] = __ldg(u.bias_values + r * u.bias_ld + j);
-        atomicOr(&sm.taken[at >> 5], 1u << (at & 31));
+    }
+    int bat[kBiasPer];
+    if (nbias) {
+#pragma unroll
+      for (int i = 0; i < kBiasPer; ++i) {
+        bat[i] = bid[i] - p0;
+        if (!in(bat[i])) {
+          bat[i] = -1;
+          continue;
+        }
+        const uint32_t bit = 1u << (bat[i] & 31);
+        if (atomicOr(&sm.biased[bat[i] >> 5], bit) & bit) atomicOr(&sm.twice[bat[i] >> 5], bit);
       }
-      __syncthreads();
     }
-    if (whole > 0 && !dead) {
-      dead = !mbar_wait(&sm.full, phase);
-      phase ^= 1;
-    }
+    float* x = sm.x[buf];
+    if (wait && !dead) dead = !mbar_wait(&sm.full[buf], (phase >> buf) & 1);
+    if (wait) phase ^= 1u << buf;
     __syncthreads();
-    // 3. rewrite the logits of ids that occur (those with a bias are taken already) ...
-    auto count_of = [&](int at) { return (sm.count[at >> 1] >> (16 * (at & 1))) & 0xFFFFu; };
-    for (int i = tid; i < hist; i += kThreads) {
-      const int at = local(__ldg(h + i));
-      if (at < 0) continue;
-      const uint32_t bit = 1u << (at & 31);
-      if (atomicOr(&sm.taken[at >> 5], bit) & bit) continue;
-      sm.x[at] = static_cast<float>(penalised(sm.x[at], count_of(at)));
+    // 2. rewrite
+    const int founds = hist ? sm.founds : 0;
+    for (int i = tid; i < founds; i += kThreads) {
+      const int at = sm.found[i];
+      if ((sm.biased[at >> 5] >> (at & 31)) & 1u) continue;
+      x[at] = static_cast<float>(penalised(x[at], sm.count[at]));
     }
-    // ... and of ids with biases, each by the first of its entries
-    for (int j = tid; j < hits; j += kThreads) {
-      const int at = sm.hit_id[j];
-      bool first = true;
-      for (int i = 0; i < j; ++i) first &= sm.hit_id[i] != at;
-      if (!first) continue;
-      double t = penalised(sm.x[at], hist ? count_of(at) : 0);
-      for (int i = j; i < hits; ++i)
-        if (sm.hit_id[i] == at) t += sm.hit_value[i];
-      sm.x[at] = static_cast<float>(t);
+    if (nbias) {
+#pragma unroll
+      for (int i = 0; i < kBiasPer; ++i)
+        if (bat[i] >= 0) {
+          double sum = bval[i];
+          if ((sm.twice[bat[i] >> 5] >> (bat[i] & 31)) & 1u) {
+            // the first entry of the id takes all of them, in list order
+            const int j = tid + i * kThreads;
+            bool first = true;
+            sum = 0.0;
+            for (int e = 0; e < nbias; ++e)
+              if (sm.bias_id[e] == bid[i]) {
+                first &= e >= j;
+                sum += sm.bias_value[e];
+              }
+            if (!first) continue;
+          }
+          x[bat[i]] = static_cast<float>(penalised(x[bat[i]], sm.count[bat[i]]) + sum);
+        }
     }
-    if (hist || hits) __syncthreads();
-    // 4. out
+    if (hist || nbias) __syncthreads();
+    // 3. out
+    // the quad of the largest logit so far (a NaN is in no maximum and above nothing)
+    auto choose = [&](const float4& y, int v) {
+      const float m = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
+      const bool up = m > best;
+      best = up ? m : best;
+      best_at = up ? v : best_at;
+    };
+    const int q0 = q_head(p0), q1 = q_end(p0);
 #pragma unroll
     for (int k = 0; k < kQuads; ++k) {
-      const int q = tid + k * kThreads, v = v0 + 4 * q;
-      if (q >= nq) break;
-      const float4 x = *reinterpret_cast<const float4*>(&sm.x[4 * q]);
-      float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (!((allow[k] >> e) & 1u)) y[e] = -INFINITY;
-        // ids before the row's start and behind its end are no candidates
-        if (y[e] > -INFINITY && v + e >= 0 && v + e < V) {
-          const uint32_t key = key_of(y[e]);
-          if (key > best) {
-            best = key;
-            best_at = v + e;
-          }
+      const int q = tid + k * kThreads, v = p0 + 4 * q - mis;
+      if (q < q0 || q >= q1) continue;
+      const uint32_t allow = allowed(k, v);
+      float4 y = *reinterpret_cast<const float4*>(x + 4 * q);
+      if (!(allow & 1u)) y.x = -INFINITY;
+      if (!(allow & 2u)) y.y = -INFINITY;
+      if (!(allow & 4u)) y.z = -INFINITY;
+      if (!(allow & 8u)) y.w = -INFINITY;
+      choose(y, v);
+      if (vec_out) {
+        *reinterpret_cast<float4*>(y_row + v) = y;
+      } else {
+        y_row[v] = y.x;
+        y_row[v + 1] = y.y;
+        y_row[v + 2] = y.z;
+        y_row[v + 3] = y.w;
+      }
+    }
+    if (tid < 8 && (tid < 4 ? q0 > 0 : q1 < nq)) {  // the cut quads, an id a thread
+      const int i = 4 * (tid < 4 ? 0 : nq - 1) + (tid & 3), v = p0 + i - mis;
+      if (v >= 0 && v < V) {
+        const bool ok = !mask || ((__ldg(mask + (v >> 5)) >> (v & 31)) & 1u);
+        const float y = ok ? x[i] : -INFINITY;
+        y_row[v] = y;
+        if (y > best || (y == best && y > -INFINITY && v < best_at)) {
+          best = y;
+          best_at = v;
         }
       }
-      if (vec_out && v >= 0 && v + 3 < V) {
-        *reinterpret_cast<float4*>(y_row + v) = make_float4(y[0], y[1], y[2], y[3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v + e >= 0 && v + e < V) y_row[v + e] = y[e];
-      }
     }
-    __syncthreads();  // the next slice reuses the shared memory
+    if (p0 + step < end) {  // counters and bits back to zero
+      for (int i = tid; i < founds; i += kThreads) sm.count[sm.found[i]] = 0;
+      if (tid == 0) sm.founds = 0;
+      if (nbias) {
+#pragma unroll
+        for (int i = 0; i < kBiasPer; ++i)
+          if (bat[i] >= 0) sm.biased[bat[i] >> 5] = sm.twice[bat[i] >> 5] = 0;
+      }
+      __syncthreads();
+    }
   }
 
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (!token) return;
   // the largest key, and the lowest id that has it
-  const uint32_t wk = __reduce_max_sync(0xffffffffu, best);
-  const uint32_t wa = __reduce_min_sync(0xffffffffu, best == wk ? best_at : 0xFFFFFFFFu);
+  uint32_t at = 0xFFFFFFFFu;
+  if (best > -INFINITY) {  // which of the quad, as this thread wrote it
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+      const int v = best_at + e;
+      if (v >= 0 && v < V && y_row[v] == best) at = v;
+    }
+  }
+  const uint32_t mine = best > -INFINITY ? key_of(best) : 0u;  // 0: nothing above -inf
+  const uint32_t wk = __reduce_max_sync(0xffffffffu, mine);
+  const uint32_t wa = __reduce_min_sync(0xffffffffu, mine == wk ? at : 0xFFFFFFFFu);
   if (lane == 0) {
     sm.best_key[warp] = wk;
     sm.best_at[warp] = wa;
@@ -241,12 +337,17 @@ __global__ __launch_bounds__(kThreads) void k_logits(const float* __restrict__ l
     const uint32_t ca = __reduce_min_sync(0xffffffffu, k == ck ? a : 0xFFFFFFFFu);
     if (lane == 0) {
       uint32_t dst;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.cluster_best[rank])), "r"(0));
-      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst), "r"(ck), "r"(ca) : "memory");
+      asm("mapa.shared::cluster.u32 %0, %1, %2;"
+          : "=r"(dst)
+          : "r"(smem_u32(&sm.cluster_best[rank])), "r"(0));
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst), "r"(ck), "r"(ca)
+                   : "memory");
     }
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (rank == 0 && tid == 0) {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (rank != 0) return;
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid == 0) {
     uint32_t k = 0, a = 0;
     for (int i = 0; i < cluster; ++i) {
       const uint2 o = sm.cluster_best[i];
@@ -264,14 +365,40 @@ __global__ __launch_bounds__(kThreads) void k_logits(const float* __restrict__ l
 cudaError_t launch_logits_process(const float* logits, int rows, int vocab,
                                   const obn_logit_rules& rules, float* out, int32_t* token,
                                   cudaStream_t s) {
-  // CTAs of a row: one per 16384 ids, and more while they would leave SMs idle.
-  int cluster = 1;
-  while (cluster < kMaxCluster &&
-         (static_cast<long long>(cluster) * kSliceIds < vocab ||
-          (static_cast<long long>(rows) * cluster < 148 && cluster * 2048 < vocab)))
-    cluster *= 2;
+  // Clusters of 16 are beyond the portable size: their place is checked once per device.
   cudaError_t e = allow_smem<&k_logits>(sizeof(LogitSmem));
   if (e != cudaSuccess) return e;
+  static std::atomic<int> largest[64];  // per device, 0: not known yet
+  int dev = 0;
+  e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int most = dev < 64 ? largest[dev].load(std::memory_order_relaxed) : 8;
+  if (most == 0) {
+    most = 8;
+    if (cudaFuncSetAttribute(k_logits, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
+        cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(kMaxCluster, 1);
+      cfg.blockDim = kThreads;
+      cfg.dynamicSmemBytes = sizeof(LogitSmem);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = kMaxCluster;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, k_logits, &cfg) == cudaSuccess && n > 0)
+        most = kMaxCluster;
+    }
+    cudaGetLastError();
+    largest[dev].store(most, std::memory_order_relaxed);
+  }
+  // As many CTAs to a row as find room at once, two on an SM.
+  const int slices = (vocab + kSliceIds - 1) / kSliceIds;
+  int cluster = 1;
+  while (cluster < most && cluster < slices && rows * cluster * 2ll <= 2 * num_sms_cached())
+    cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, rows);
   cfg.blockDim = kThreads;
@@ -286,7 +413,7 @@ cudaError_t launch_logits_process(const float* logits, int rows, int vocab,
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_logits, logits, vocab, rules, cluster, out, token);
+  return cudaLaunchKernelEx(&cfg, k_logits, logits, vocab, rules, out, token);
 }
 
 }  // namespace obn
