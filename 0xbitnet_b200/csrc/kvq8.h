@@ -46,6 +46,12 @@ cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, 
                                 const int* lens_dev, float scale, float* out, void* workspace,
                                 cudaStream_t s);
 
+// Its pass for tiles of 256 query rows (kvq8_many.cu), and what that pass needs.
+size_t attention_q8_many_workspace_bytes();
+cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, int H, int seq_len,
+                                     const int* lens_dev, float scale_log2, float* out, void* ws,
+                                     cudaStream_t s);
+
 // Launch with programmatic dependent launch allowed.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,

@@ -31,9 +31,7 @@
 #include <cfloat>
 #include <cmath>
 
-#include "gemm.h"
 #include "kvq8_sched.cuh"
-#include "tc05.cuh"
 
 namespace obn {
 
@@ -74,37 +72,11 @@ OBN_DEVINL void mma_su8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-OBN_DEVINL float shx(float v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
-OBN_DEVINL uint32_t shxu(uint32_t v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
-OBN_DEVINL float ex2(float x) {  // 2^x; results below 2^-126 become 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // An overflowed score stays the largest or smallest number, a NaN stays one.
 OBN_DEVINL float clamp_score(float x) {
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(FLT_MAX));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-FLT_MAX));
   return x;
-}
-
-// Codes of 4 keys (rows r) x 4 dims -> 4 dims x 4 keys.
-OBN_DEVINL void transpose4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&o)[4]) {
-  const uint32_t a = __byte_perm(r0, r1, 0x5140), b = __byte_perm(r0, r1, 0x7362);
-  const uint32_t c = __byte_perm(r2, r3, 0x5140), d = __byte_perm(r2, r3, 0x7362);
-  o[0] = __byte_perm(a, c, 0x5410);
-  o[1] = __byte_perm(a, c, 0x7632);
-  o[2] = __byte_perm(b, d, 0x5410);
-  o[3] = __byte_perm(b, d, 0x7632);
-}
-
-OBN_DEVINL void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
-                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
-      "{%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
 }
 
 OBN_DEVINL void cp_async4(uint32_t dst, const float* src, bool in) {  // zeros when !in
@@ -559,22 +531,6 @@ __global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, float* 
   *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
-// The codes as a 4-D tensor (128 dims, KV heads, positions, sequences), boxes of `rows`
-// positions of one head, 128-byte swizzle; rows past S_max read as zeros.
-bool q8_map(CUtensorMap* map, const int8_t* codes, const Q8Cache& c, int rows) {
-  const cuuint64_t row = static_cast<cuuint64_t>(c.Hkv) * D;
-  const cuuint64_t dims[4] = {D, static_cast<cuuint64_t>(c.Hkv), static_cast<cuuint64_t>(c.S_max),
-                              static_cast<cuuint64_t>(c.B)};
-  const cuuint64_t strides[3] = {D, row, row * c.S_max};
-  const cuuint32_t box[4] = {D, 1, static_cast<cuuint32_t>(rows), 1};
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  auto fn = tensor_map_encoder();
-  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(codes), dims, strides,
-                  box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int MT, int KW, int ST, int CTAS>
 cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale_log2, float* out,
                        float* ws, cudaStream_t s) {
@@ -597,9 +553,13 @@ cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale
 
 }  // namespace
 
+// Query rows of a sequence and KV head up to which the few-rows pass runs.
+constexpr int kFewRows = 32;
+
 size_t attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int S_max) {
-  (void)B, (void)n, (void)H, (void)Hkv, (void)S_max;
-  return q8_workspace(16);
+  (void)B, (void)S_max;
+  const long long rows = static_cast<long long>(n) * (H / Hkv);
+  return rows > kFewRows ? attention_q8_many_workspace_bytes() : q8_workspace(16, kQ8MaxCtas);
 }
 
 cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, int seq_len,
@@ -608,6 +568,8 @@ cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, 
   Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, 0, 0, seq_len, lens_dev, 0};
   const long long rows = static_cast<long long>(n) * sc.G;
   const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  if (rows > kFewRows)
+    return launch_attention_q8_many(q, c, n, H, seq_len, lens_dev, scale_log2, out, workspace, s);
   sc.tile_rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
   sc.tiles = static_cast<int>((rows + sc.tile_rows - 1) / sc.tile_rows);
   float* ws = static_cast<float*>(workspace);

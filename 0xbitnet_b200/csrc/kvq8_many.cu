@@ -1,0 +1,585 @@
+// kvq8_many.cu — attention over the 8-bit KV cache for many query rows (prefill chunks).
+//
+// Here the tensor cores bound the pass: 4 * 128 operations per query row and key. They run as
+// tcgen05.mma kind::f16 with f32 accumulators in tensor memory. The codes are whole numbers up
+// to 127 and exact in f16; q and the weights are f32, so each is an f16 high part and the f16 of
+// what is left (x = hi + lo to 2^-22), two MMAs for one. (kind::i8 has twice the rate, but
+// three digits and an s32 accumulator for each of them: more tensor memory than there is.)
+//
+// One CTA per SM works on a pair of tiles, 2 x 128 query rows (token, group head) of a sequence
+// and KV head, so every converted key block serves 256 rows, and on units of 128 keys
+// (kvq8_sched.cuh). Roles, 13 warps:
+//   warps 0-3, 4-7  softmax of tile A, B: a thread is a row. S from tensor memory twice (maximum;
+//                   weights), the weights back over S as the A operand of the second product.
+//   warps 8-11      codes to f16: TMA staging -> registers -> shared memory in the MMA's layout;
+//                   V is transposed on the way. The staging is requested again as soon as
+//                   it is read.
+//   warp 12         issues the MMAs, in the order  PV_A(u) QK_A(u+1) PV_B(u) QK_B(u+1): while
+//                   one tile's softmax runs, the other tile's products do.
+// Tensor memory: S (and P) of A and B, 2 x 128 columns, O of A and B, 2 x 128.
+//
+// Softmax. With s = q.k, f = scale of q, key block and log2 e, v's block scale 2^lv: a weight
+// is w = 2^(s f + lv - R), so its f16 pair is as exact as the contribution it makes is large,
+// whatever the scales of other blocks, and O adds w times codes. R moves only when a row's
+// maximum of s f + lv exceeds it by 15 (w <= 2^15 fits f16); then O is rescaled in
+// tensor memory. The total is the sum of w 2^(lv0 - lv), exact factors, lv0 fixed for a part.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include <cuda_fp16.h>
+
+#include "kvq8_sched.cuh"
+
+namespace obn {
+
+int num_sms_cached();  // kernels.cu
+
+namespace {
+
+constexpr int D = kQ8HeadDim;
+constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
+constexpr int kThreads = 416;
+constexpr int kManyMaxCtas = 160;
+constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
+
+struct ManySmem {
+  uint8_t q[2][2][2 * kHalf];  // [tile][hi, lo][dims 0-63, 64-127]
+  uint8_t k[2 * kHalf];        // 128 keys x 128 dims
+  uint8_t v[2 * kHalf];        // 128 dims x 128 keys
+  uint8_t k_in[kUnitKeys * D], v_in[kUnitKeys * D];
+  uint64_t kin_full, vin_full, kin_read, vin_read;
+  uint64_t k_full, k_free, v_full, v_free;
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+  long long sh[kThreads / 32 + 8];
+};
+static_assert(sizeof(ManySmem) <= 227 * 1024, "shared memory");
+
+constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(128 >> 3) << 17) |
+                            (static_cast<uint32_t>(128 >> 4) << 24);  // f32 = f16 x f16, 128 x 128
+
+// A from tensor memory.
+OBN_DEVINL void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(kIdesc), "r"(accumulate)
+      : "memory");
+}
+
+// The key at position (row of K, k index of V) r of a unit: within a group of 8 keys a the
+// order is rotated by a, which keeps the transposing loads of V free of bank conflicts.
+OBN_DEVINL int key_at(int r) { return (r & ~7) | ((r + (r >> 3)) & 7); }
+
+// Four signed bytes -> f16: 1024 + (c + 128) in the low mantissa bits, minus 1152.
+OBN_DEVINL void bytes_to_half(uint32_t w, uint32_t* h01, uint32_t* h23) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), off);
+  __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+  *h01 = *reinterpret_cast<uint32_t*>(&ha);
+  *h23 = *reinterpret_cast<uint32_t*>(&hb);
+}
+
+__global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
+    const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+    const float* __restrict__ q, const float* __restrict__ k_scale,
+    const float* __restrict__ v_scale, int nblk, Q8Sched sc, float scale_log2,
+    float* __restrict__ out, float* __restrict__ ws) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  ManySmem* sm = reinterpret_cast<ManySmem*>(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    mbar_init(&sm->kin_full, 1);
+    mbar_init(&sm->vin_full, 1);
+    mbar_init(&sm->kin_read, 128);
+    mbar_init(&sm->vin_read, 128);
+    mbar_init(&sm->k_full, 128);
+    mbar_init(&sm->k_free, 1);
+    mbar_init(&sm->v_full, 128);
+    mbar_init(&sm->v_free, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sm->q_full[x], 128);
+      mbar_init(&sm->s_full[x], 1);
+      mbar_init(&sm->p_full[x], 128);
+      mbar_init(&sm->o_full[x], 1);
+    }
+    mbar_init(&sm->drain, 1);
+    sm->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&sm->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm->tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
+  Q8Cursor cur = q8_share<kThreads>(sc, sm->sh);
+
+  if (cur.left == 0) {
+    // nothing for this CTA
+  } else if (warp < 8) {
+    // ---- softmax: thread = row `row` of tile x ------------------------------------------
+    const int x = warp >> 2, row = tid & 127;
+    const int H = sc.G * sc.Hkv, rows_seq = sc.n * sc.G;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + 128 * x, t_o = tmem + lane_base + 256 + 128 * x;
+    float R = -INFINITY, l = 0.0f, lv0 = 0.0f, sq = 0.0f, scl = 0.0f;
+    int lim = 0, u_first = 0, r = 0;
+    size_t row_off = 0;  // of this row in q and out, in floats
+    bool fresh = true, ok = true;
+    // lanes 0-7: the unit's key scales, 8-15: its value scales
+    auto load_scale = [&](const Q8Cursor& c) {
+      const int blk = c.unit * (kUnitKeys / kQ8Block) + (lane & 7);
+      return lane < 16 && blk * kQ8Block < c.len
+                 ? __ldg((lane < 8 ? k_scale : v_scale) +
+                         (static_cast<size_t>(c.b) * nblk + blk) * sc.Hkv + c.kvh)
+                 : 0.0f;
+    };
+    scl = load_scale(cur);
+    for (int u = 0; cur.left > 0; ++u) {
+      const int k0 = cur.unit * kUnitKeys;
+      Q8Cursor nxt = cur;
+      q8_next(sc, nxt);
+      if (fresh) {  // this row of q as f16 hi and lo, scaled to below 2^14
+        u_first = cur.unit;
+        r = cur.tile * kRows + 128 * x + row;
+        const bool real = r < rows_seq;
+        const int t = real ? r / sc.G : 0, g = real ? r - t * sc.G : 0;
+        row_off = ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D;
+        const float4* src = reinterpret_cast<const float4*>(q + row_off);
+        uint32_t big = 0;
+        if (real) {
+#pragma unroll 8
+          for (int i = 0; i < D / 4; ++i) {
+            const float4 y = __ldg(src + i);
+            big = max(big, max(max(__float_as_uint(y.x) & 0x7FFFFFFFu, __float_as_uint(y.y) & 0x7FFFFFFFu),
+                               max(__float_as_uint(y.z) & 0x7FFFFFFFu, __float_as_uint(y.w) & 0x7FFFFFFFu)));
+          }
+        }
+        const bool bad = big >= 0x7F800000u;
+        const int ex = max(static_cast<int>(big >> 23) - 126, -90);  // |q| < 2^ex
+        const float up = __int_as_float((127 + 14 - ex) << 23);
+        sq = (bad ? __int_as_float(0x7FC00000) : __int_as_float((127 + ex - 14) << 23)) * scale_log2;
+        uint8_t* hi = sm->q[x][0] + row * 128;
+        uint8_t* lo = sm->q[x][1] + row * 128;
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          float e[8] = {};
+          if (real && !bad) {
+            const float4 a = __ldg(src + 2 * i), b = __ldg(src + 2 * i + 1);
+            e[0] = a.x * up, e[1] = a.y * up, e[2] = a.z * up, e[3] = a.w * up;
+            e[4] = b.x * up, e[5] = b.y * up, e[6] = b.z * up, e[7] = b.w * up;
+          }
+          uint4 wh, wl;
+          uint32_t* ph = &wh.x;
+          uint32_t* pl = &wl.x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
+            const float2 hf = __half22float2(h);
+            const __half2 m = __floats2half2_rn(e[2 * j] - hf.x, e[2 * j + 1] - hf.y);
+            ph[j] = *reinterpret_cast<const uint32_t*>(&h);
+            pl[j] = *reinterpret_cast<const uint32_t*>(&m);
+          }
+          const int at = (i >> 3) * kHalf + (((i & 7) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(hi + at) = wh;
+          *reinterpret_cast<uint4*>(lo + at) = wl;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&sm->q_full[x]);
+        lim = real ? min(cur.len, q8_limit(sc, cur.len, r)) : 0;
+        R = -INFINITY;
+        l = 0.0f;
+        // the reference of the value scales: the unit's largest exponent
+        float top = lane >= 8 && lane < 16 && scl > 0.0f ? scl : 0.0f;
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        lv0 = top > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127) : 0.0f;
+      }
+      // exponents of the value scales (of zero and poisoned blocks: any, the weights of a zero
+      // one are left out of P and count in the total) and what poisons a total: 0, or NaN
+      const bool plain = scl > 0.0f;
+      const float lv_lane =
+          plain ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127) : lv0;
+      const float bad_lane = scl - scl;
+      const uint32_t zero = __ballot_sync(0xffffffffu, scl == 0.0f) >> 8;
+      const float scl_now = scl;
+      if (nxt.left > 0) scl = load_scale(nxt);
+
+      ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->s_full[x], u & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const bool all = __all_sync(0xffffffffu, k0 + kUnitKeys <= lim);  // nothing masked
+      const int seen = lim - k0;  // keys of the unit that this row sees
+      // 1. the largest s f + lv
+      float xr = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld32(t_s + 32 * c, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {
+          const int b = 2 * c + hb;
+          const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
+          const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
+          float m = -INFINITY;
+          if (all) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(s[16 * hb + i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              m = fmaxf(m, key_at(16 * b + i) < seen ? __uint_as_float(s[16 * hb + i]) : -INFINITY);
+          }
+          xr = fmaxf(xr, m == -INFINITY ? -INFINITY : fmaf(m, f, lv));
+        }
+      }
+      const bool grow = xr > R + 15.0f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float Rn = grow ? ceilf(xr) - 7.0f : R;
+        const float corr = grow ? ex2(R - Rn) : 1.0f;
+        l *= corr;
+        R = Rn;
+        if (!fresh) {  // O holds sums of this part
+          ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->o_full[x], (u - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st32(t_o + 32 * c, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      fresh = false;
+      // 2. the weights, over the scores: 8 columns of high and 8 of low halves per 16 keys
+      const float Rs = R == -INFINITY ? 0.0f : R;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld32(t_s + 32 * c, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {
+          const int b = 2 * c + hb;
+          const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
+          const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
+          const float poison = __shfl_sync(0xffffffffu, bad_lane, 8 + b);
+          const float base = lv - Rs;
+          float w[16], sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            w[i] = ex2(fmaf(__uint_as_float(s[16 * hb + i]), f, base));
+            if (!all) w[i] = key_at(16 * b + i) < seen ? w[i] : 0.0f;
+            sum += w[i];
+          }
+          if (16 * b < seen) l += sum * ex2(fminf(fmaxf(lv0 - lv, -126.0f), 126.0f)) + poison;
+          if ((zero >> b) & 1u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+            const float2 hf = __half22float2(h);
+            const __half2 m = __floats2half2_rn(w[2 * i] - hf.x, w[2 * i + 1] - hf.y);
+            s[16 * hb + i] = *reinterpret_cast<const uint32_t*>(&h);
+            s[16 * hb + 8 + i] = *reinterpret_cast<const uint32_t*>(&m);
+          }
+        }
+        tmem_st32(t_s + 32 * c, s);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm->p_full[x]);
+
+      const bool pair_ends = cur.unit + 1 == cur.units;
+      if (pair_ends || nxt.left == 0) {  // write the pair or its part
+        ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->o_full[x], u & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const bool whole = pair_ends && u_first == 0;
+        const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
+        const float unit = ex2(lv0) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+        float* dst = whole ? out + row_off : q8_part_o(ws, kRows, slot) + (128 * x + row) * D;
+        if (!whole) {
+          float* ml = q8_part_ml(ws, kRows, slot);
+          ml[128 * x + row] = R == -INFINITY ? -INFINITY : R - lv0;
+          ml[kRows + 128 * x + row] = l;
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_ld_wait();
+          if (r < rows_seq) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) =
+                  make_float4(__uint_as_float(o[4 * i]) * unit, __uint_as_float(o[4 * i + 1]) * unit,
+                              __uint_as_float(o[4 * i + 2]) * unit, __uint_as_float(o[4 * i + 3]) * unit);
+          }
+        }
+        tc_fence_before();
+        fresh = true;
+      }
+      cur = nxt;
+    }
+  } else if (warp < 12) {
+    // ---- codes to f16 ------------------------------------------------------------------------
+    const int ct = tid - 256, cw = ct >> 5;
+    auto request = [&](const Q8Cursor& c, const CUtensorMap* map, uint8_t* dst, uint64_t* bar) {
+      const int k0 = c.unit * kUnitKeys;
+      mbar_arrive_expect_tx(bar, kUnitKeys * D);
+      tma_load_4d(smem_u32(dst), map, 0, c.kvh, k0, c.b, bar);
+    };
+    int k_asked = 0, v_asked = 0, k_got = 0, v_got = 0;
+    if (ct == 0) {
+      request(cur, &tmap_k, sm->k_in, &sm->kin_full);
+      request(cur, &tmap_v, sm->v_in, &sm->vin_full);
+      k_asked = v_asked = 1;
+    }
+    const int k_row = key_at(ct);
+    const int a = lane & 15, chunk = 2 * cw + (lane >> 4);  // V: key group, 16 dims
+    for (int u = 0; cur.left > 0; ++u) {
+      Q8Cursor nxt = cur;
+      q8_next(sc, nxt);
+      // K: row ct of the operand is key k_row
+      if (!wait_or_abort(sm, &sm->kin_full, u & 1)) break;
+      ++k_got;
+      uint4 in[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        in[c] = *reinterpret_cast<const uint4*>(sm->k_in + k_row * D + ((c ^ (k_row & 7)) << 4));
+      // the next copy writes through the async proxy: without the fence it overtook these loads
+      fence_proxy_async_smem();
+      mbar_arrive(&sm->kin_read);
+      if (ct == 0 && nxt.left > 0) {
+        if (!wait_or_abort(sm, &sm->kin_read, u & 1)) break;
+        request(nxt, &tmap_k, sm->k_in, &sm->kin_full);
+        ++k_asked;
+      }
+      if (u > 0 && !wait_or_abort(sm, &sm->k_free, (u - 1) & 1)) break;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint4 h0, h1;
+        bytes_to_half(in[c].x, &h0.x, &h0.y);
+        bytes_to_half(in[c].y, &h0.z, &h0.w);
+        bytes_to_half(in[c].z, &h1.x, &h1.y);
+        bytes_to_half(in[c].w, &h1.z, &h1.w);
+        uint8_t* dst = sm->k + (c >> 2) * kHalf + ct * 128;
+        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3)) ^ (ct & 7)) << 4)) = h0;
+        *reinterpret_cast<uint4*>(dst + (((2 * (c & 3) + 1) ^ (ct & 7)) << 4)) = h1;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sm->k_full);
+      // V: 8 keys x 16 dims, transposed
+      if (!wait_or_abort(sm, &sm->vin_full, u & 1)) break;
+      ++v_got;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int vr = 8 * a + ((i + a) & 7);
+        in[i] = *reinterpret_cast<const uint4*>(sm->v_in + vr * D + ((chunk ^ (vr & 7)) << 4));
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sm->vin_read);
+      if (ct == 0 && nxt.left > 0) {
+        if (!wait_or_abort(sm, &sm->vin_read, u & 1)) break;
+        request(nxt, &tmap_v, sm->v_in, &sm->vin_full);
+        ++v_asked;
+      }
+      if (u > 0 && !wait_or_abort(sm, &sm->v_free, (u - 1) & 1)) break;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        auto word = [&](const uint4& y) { return w == 0 ? y.x : w == 1 ? y.y : w == 2 ? y.z : y.w; };
+        uint32_t t0[4], t1[4];
+        transpose4(word(in[0]), word(in[1]), word(in[2]), word(in[3]), t0);
+        transpose4(word(in[4]), word(in[5]), word(in[6]), word(in[7]), t1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int dim = 16 * chunk + 4 * w + e;
+          uint4 h;
+          bytes_to_half(t0[e], &h.x, &h.y);
+          bytes_to_half(t1[e], &h.z, &h.w);
+          *reinterpret_cast<uint4*>(sm->v + (a >> 3) * kHalf + dim * 128 +
+                                    (((a & 7) ^ (dim & 7)) << 4)) = h;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sm->v_full);
+      cur = nxt;
+    }
+    if (ct == 0) {  // after an abort: copies that nobody waited for
+      if (k_asked > k_got) mbar_wait(&sm->kin_full, (k_asked - 1) & 1);
+      if (v_asked > v_got) mbar_wait(&sm->vin_full, (v_asked - 1) & 1);
+    }
+  } else {
+    // ---- MMAs ----------------------------------------------------------------------------------
+    const uint32_t s_q = smem_u32(sm->q[0][0]), s_k = smem_u32(sm->k), s_v = smem_u32(sm->v);
+    bool ok = true;
+    int pairs = 0;
+    // S of tile x = Q K^T for unit u; `start`: the first of a pair
+    auto qk = [&](int x, int u, bool start) {
+      if (!ok) return;
+      if (x == 0) ok = wait_or_abort(sm, &sm->k_full, u & 1);
+      if (ok && start) ok = wait_or_abort(sm, &sm->q_full[x], pairs & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int lo = 0; lo < 2; ++lo) {
+            const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
+            mma_f16(tmem + 128 * x, sw128_desc(s_q + (2 * x + lo) * 2 * kHalf + off),
+                    sw128_desc(s_k + off), kIdesc, j > 0 || lo > 0 ? 1u : 0u);
+          }
+        mma_commit(&sm->s_full[x]);
+        if (x == 1) mma_commit(&sm->k_free);
+      }
+      __syncwarp();
+    };
+    // O of tile x += P V
+    auto pv = [&](int x, int u, bool start) {
+      if (!ok) return;
+      if (x == 0) ok = wait_or_abort(sm, &sm->v_full, u & 1);
+      if (ok) ok = wait_or_abort(sm, &sm->p_full[x], u & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int lo = 0; lo < 2; ++lo) {
+            const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
+            mma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 16 * j + 8 * lo, sw128_desc(s_v + off),
+                       !start || j > 0 || lo > 0 ? 1u : 0u);
+          }
+        mma_commit(&sm->o_full[x]);
+        if (x == 1) mma_commit(&sm->v_free);
+      }
+      __syncwarp();
+    };
+    qk(0, 0, true);
+    qk(1, 0, true);
+    bool start = true;
+    for (int u = 0; cur.left > 0 && ok; ++u) {
+      const bool pair_ends = cur.unit + 1 == cur.units;
+      q8_next(sc, cur);
+      const bool more = cur.left > 0;
+      pv(0, u, start);
+      if (more && !pair_ends) qk(0, u + 1, false);
+      pv(1, u, start);
+      if (more && !pair_ends) qk(1, u + 1, false);
+      if (more && pair_ends) {
+        ++pairs;
+        qk(0, u + 1, true);
+        qk(1, u + 1, true);
+      }
+      start = pair_ends;
+    }
+    if (lane == 0) mma_commit(&sm->drain);
+    __syncwarp();
+    mbar_wait(&sm->drain, 0);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// k_q8_join for tiles of many rows: a warp per row, few parts each.
+__global__ __launch_bounds__(256) void k_q8_join_rows(Q8Sched sc, float* __restrict__ ws,
+                                                      float* __restrict__ out) {
+  __shared__ long long sh[8 + 1];
+  constexpr int kPer = 32;  // rows of a CTA
+  const int groups = sc.tile_rows / kPer;
+  const int item = blockIdx.x / groups, r0 = blockIdx.x % groups * kPer, kvh = blockIdx.y;
+  const int b = item / sc.tiles, tile = item - b * sc.tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int units = q8_units(sc, item);
+  long long front;
+  const long long total = q8_locate<256>(sc, item, &front, sh);
+  int c0 = 0, c1 = 0;
+  if (units) {
+    const long long x0 = front + static_cast<long long>(kvh) * (units + 1) + 1;  // unit 0
+    const int ctas = q8_ctas(sc, total);
+    c0 = q8_owner(total, ctas, x0);
+    c1 = q8_owner(total, ctas, x0 + units - 1);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (units && c0 == c1) return;  // written by its CTA
+  for (int i = warp; i < kPer; i += 8) {
+    const int row = r0 + i, r = tile * sc.tile_rows + row;
+    if (r >= sc.n * sc.G) return;
+    const int t = r / sc.G, g = r - t * sc.G;
+    float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D + 4 * lane;
+    float m = -INFINITY, l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (units) {
+      for (int c = c0; c <= c1; ++c) {
+        const int slot = 2 * c + (c == c0 ? 1 : 0);
+        const float* ml = q8_part_ml(ws, sc.tile_rows, slot);
+        const float pm = ml[row], pl = ml[sc.tile_rows + row];
+        const float4 x = *reinterpret_cast<const float4*>(
+            q8_part_o(ws, sc.tile_rows, slot) + static_cast<size_t>(row) * D + 4 * lane);
+        const float mn = fmaxf(m, pm);
+        // a part without keys, or of NaN scores only, has -inf here
+        const float e0 = m == mn ? 1.0f : ex2(m - mn), e1 = pm == mn ? 1.0f : ex2(pm - mn);
+        l = l * e0 + pl * e1;
+        y = make_float4(y.x * e0 + x.x * e1, y.y * e0 + x.y * e1, y.z * e0 + x.z * e1,
+                        y.w * e0 + x.w * e1);
+        m = mn;
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  }
+}
+
+}  // namespace
+
+size_t attention_q8_many_workspace_bytes() { return q8_workspace(kRows, kManyMaxCtas); }
+
+cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, int H, int seq_len,
+                                     const int* lens_dev, float scale_log2, float* out, void* ws,
+                                     cudaStream_t s) {
+  Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, kRows, 0, seq_len, lens_dev, 0};
+  const long long rows = static_cast<long long>(n) * sc.G;
+  sc.tiles = static_cast<int>((rows + kRows - 1) / kRows);
+  cudaError_t e = allow_smem<&k_attn_q8_many>(sizeof(ManySmem));
+  if (e != cudaSuccess) return e;
+  CUtensorMap mk, mv;
+  if (!q8_map(&mk, c.k, c, kUnitKeys) || !q8_map(&mv, c.v, c, kUnitKeys))
+    return cudaErrorNotSupported;
+  const long long bound = static_cast<long long>(sc.B) * sc.tiles * sc.Hkv *
+                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys + 1);
+  sc.ctas = static_cast<int>(
+      std::max<long long>(std::min<long long>(bound, std::min(num_sms_cached(), kManyMaxCtas)), 1));
+  e = launch_pdl(&k_attn_q8_many, dim3(sc.ctas), kThreads, sizeof(ManySmem), s, mk, mv, q, c.k_scale,
+                 c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, static_cast<float*>(ws));
+  if (e != cudaSuccess) return e;
+  return launch_pdl(&k_q8_join_rows, dim3(sc.B * sc.tiles * (kRows / 32), sc.Hkv), 256, 0, s, sc,
+                    static_cast<float*>(ws), out);
+}
+
+}  // namespace obn

@@ -9,12 +9,14 @@
 // mix of lengths and causal tiles of any depth keep every CTA equally busy, and one long
 // sequence is split as finely as many short ones. A pair that lies inside one CTA is written
 // out by it; the parts of a pair that spans CTAs go to the workspace and are joined by
-// k_q8_join. A CTA holds at most two parts: one that continues a pair (slot 2c) and one that
+// k_q8_join (or k_q8_join_rows). A CTA holds at most two parts: one that continues a pair (slot 2c) and one that
 // begins a pair and does not end it (slot 2c + 1).
 #pragma once
 
+#include "gemm.h"
 #include "kvq8.h"
 #include "obn_common.cuh"
+#include "tc05.cuh"
 
 namespace obn {
 
@@ -206,6 +208,48 @@ OBN_DEVINL void q8_next(const Q8Sched& s, Q8Cursor& c) {
   q8_enter(s, c);
 }
 
+OBN_DEVINL float shx(float v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
+OBN_DEVINL uint32_t shxu(uint32_t v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
+OBN_DEVINL float ex2(float x) {  // 2^x; results below 2^-126 become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Codes of 4 keys (rows r) x 4 dims -> 4 dims x 4 keys.
+OBN_DEVINL void transpose4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&o)[4]) {
+  const uint32_t a = __byte_perm(r0, r1, 0x5140), b = __byte_perm(r0, r1, 0x7362);
+  const uint32_t c = __byte_perm(r2, r3, 0x5140), d = __byte_perm(r2, r3, 0x7362);
+  o[0] = __byte_perm(a, c, 0x5410);
+  o[1] = __byte_perm(a, c, 0x7632);
+  o[2] = __byte_perm(b, d, 0x5410);
+  o[3] = __byte_perm(b, d, 0x7632);
+}
+
+OBN_DEVINL void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The codes as a 4-D tensor (128 dims, KV heads, positions, sequences), boxes of `rows`
+// positions of one head, 128-byte swizzle; rows past S_max read as zeros.
+inline bool q8_map(CUtensorMap* map, const int8_t* codes, const Q8Cache& c, int rows) {
+  const cuuint64_t row = static_cast<cuuint64_t>(c.Hkv) * kQ8HeadDim;
+  const cuuint64_t dims[4] = {kQ8HeadDim, static_cast<cuuint64_t>(c.Hkv), static_cast<cuuint64_t>(c.S_max),
+                              static_cast<cuuint64_t>(c.B)};
+  const cuuint64_t strides[3] = {kQ8HeadDim, row, row * c.S_max};
+  const cuuint32_t box[4] = {kQ8HeadDim, 1, static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  auto fn = tensor_map_encoder();
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(codes), dims, strides,
+                  box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Workspace of a pass of `rows` rows per tile: for each of 2 C slots the sums [rows][128],
 // then the maxima and totals [rows] (all f32).
 OBN_DEVINL float* q8_part_o(float* ws, int rows, int slot) {
@@ -214,8 +258,8 @@ OBN_DEVINL float* q8_part_o(float* ws, int rows, int slot) {
 OBN_DEVINL float* q8_part_ml(float* ws, int rows, int slot) {
   return q8_part_o(ws, rows, slot) + static_cast<size_t>(rows) * kQ8HeadDim;
 }
-inline size_t q8_workspace(int rows) {
-  return static_cast<size_t>(2) * kQ8MaxCtas * rows * (kQ8HeadDim + 2) * sizeof(float);
+inline size_t q8_workspace(int rows, int ctas) {
+  return static_cast<size_t>(2) * ctas * rows * (kQ8HeadDim + 2) * sizeof(float);
 }
 
 }  // namespace obn
