@@ -75,6 +75,18 @@ OBN_DEVINL void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uin
 // order is rotated by a, which keeps the transposing loads of V free of bank conflicts.
 OBN_DEVINL int key_at(int r) { return (r & ~7) | ((r + (r >> 3)) & 7); }
 
+// The same for column i of the 32 columns from 32 c on, against their first key.
+OBN_DEVINL int key_in_32(int i, int c) { return (i & ~7) | ((i + (i >> 3) + 4 * c) & 7); }
+
+OBN_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
 // Four signed bytes -> f16: 1024 + (c + 128) in the low mantissa bits, minus 1152.
 OBN_DEVINL void bytes_to_half(uint32_t w, uint32_t* h01, uint32_t* h23) {
   const uint32_t u = w ^ 0x80808080u;
@@ -215,34 +227,39 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       const float scl_now = scl;
       if (nxt.left > 0) scl = load_scale(nxt);
 
-      ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->s_full[x], u & 1));
+      const int seen = lim - k0;  // keys of the unit that this row sees
+      const bool all = __all_sync(0xffffffffu, seen >= kUnitKeys);  // nothing masked
+      ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->s_full[x], u & 1));
       if (!ok) break;
       tc_fence_after();
-      const bool all = __all_sync(0xffffffffu, k0 + kUnitKeys <= lim);  // nothing masked
-      const int seen = lim - k0;  // keys of the unit that this row sees
-      // 1. the largest s f + lv
+      // 1. the largest s f + lv. The loops over 16-key blocks stay loops: unrolled, the two softmax
+      // groups, the converters and the MMA warp evict each other's instructions (both passes
+      // unrolled fully: 8600 cycles a unit; in halves: 5600).
       float xr = -INFINITY;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t s[32];
         tmem_ld32(t_s + 32 * c, s);
+        const float f0 = sq * __shfl_sync(0xffffffffu, scl_now, 2 * c);
+        const float f1 = sq * __shfl_sync(0xffffffffu, scl_now, 2 * c + 1);
+        const float lv_0 = __shfl_sync(0xffffffffu, lv_lane, 8 + 2 * c);
+        const float lv_1 = __shfl_sync(0xffffffffu, lv_lane, 9 + 2 * c);
         tmem_ld_wait();
+        if (!all) {
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {
-          const int b = 2 * c + hb;
-          const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
-          const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
-          float m = -INFINITY;
-          if (all) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(s[16 * hb + i]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              m = fmaxf(m, key_at(16 * b + i) < seen ? __uint_as_float(s[16 * hb + i]) : -INFINITY);
-          }
-          xr = fmaxf(xr, m == -INFINITY ? -INFINITY : fmaf(m, f, lv));
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + key_in_32(i, c) >= seen) s[i] = 0xFF800000u;  // -inf
         }
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = __uint_as_float(s[8 * i]);
+#pragma unroll
+          for (int j = 1; j < 8; ++j) m[i] = fmaxf(m[i], __uint_as_float(s[8 * i + j]));
+        }
+        const float m0 = fmaxf(m[0], m[1]), m1 = fmaxf(m[2], m[3]);
+        xr = fmaxf(xr, m0 == -INFINITY ? -INFINITY : fmaf(m0, f0, lv_0));
+        xr = fmaxf(xr, m1 == -INFINITY ? -INFINITY : fmaf(m1, f1, lv_1));
       }
       const bool grow = xr > R + 15.0f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -251,7 +268,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         l *= corr;
         R = Rn;
         if (!fresh) {  // O holds sums of this part
-          ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->o_full[x], (u - 1) & 1));
+          ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -269,40 +286,42 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       fresh = false;
       // 2. the weights, over the scores: 8 columns of high and 8 of low halves per 16 keys
       const float Rs = R == -INFINITY ? 0.0f : R;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_ld32(t_s + 32 * c, s);
+#pragma unroll 1
+      for (int b = 0; b < 8; ++b) {
+        uint32_t s[16];
+        tmem_ld16(t_s + 16 * b, s);
+        const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
+        const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
+        const float poison = __shfl_sync(0xffffffffu, bad_lane, 8 + b);
+        const float base = lv - Rs;
         tmem_ld_wait();
+        float w[16];
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {
-          const int b = 2 * c + hb;
-          const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
-          const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
-          const float poison = __shfl_sync(0xffffffffu, bad_lane, 8 + b);
-          const float base = lv - Rs;
-          float w[16], sum = 0.0f;
+        for (int i = 0; i < 16; ++i) w[i] = ex2(fmaf(__uint_as_float(s[i]), f, base));
+        if (!all) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[i] = ex2(fmaf(__uint_as_float(s[16 * hb + i]), f, base));
-            if (!all) w[i] = key_at(16 * b + i) < seen ? w[i] : 0.0f;
-            sum += w[i];
-          }
-          if (16 * b < seen) l += sum * ex2(fminf(fmaxf(lv0 - lv, -126.0f), 126.0f)) + poison;
-          if ((zero >> b) & 1u) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
-            const float2 hf = __half22float2(h);
-            const __half2 m = __floats2half2_rn(w[2 * i] - hf.x, w[2 * i + 1] - hf.y);
-            s[16 * hb + i] = *reinterpret_cast<const uint32_t*>(&h);
-            s[16 * hb + 8 + i] = *reinterpret_cast<const uint32_t*>(&m);
-          }
+          for (int i = 0; i < 16; ++i)
+            if (32 * (b >> 1) + key_in_32(16 * (b & 1) + i, b >> 1) >= seen) w[i] = 0.0f;
         }
-        tmem_st32(t_s + 32 * c, s);
+        float sum[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = (w[i] + w[i + 4]) + (w[i + 8] + w[i + 12]);
+        if (16 * b < seen)
+          l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) *
+                   ex2(fminf(fmaxf(lv0 - lv, -126.0f), 126.0f)) + poison;
+        if ((zero >> b) & 1u) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+          const float2 hf = __half22float2(h);
+          const __half2 m = __floats2half2_rn(w[2 * i] - hf.x, w[2 * i + 1] - hf.y);
+          s[i] = *reinterpret_cast<const uint32_t*>(&h);
+          s[8 + i] = *reinterpret_cast<const uint32_t*>(&m);
+        }
+        tmem_st16(t_s + 16 * b, s);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -310,7 +329,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
 
       const bool pair_ends = cur.unit + 1 == cur.units;
       if (pair_ends || nxt.left == 0) {  // write the pair or its part
-        ok = __all_sync(0xffffffffu, wait_or_abort(sm, &sm->o_full[x], u & 1));
+        ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], u & 1));
         if (!ok) break;
         tc_fence_after();
         const bool whole = pair_ends && u_first == 0;
@@ -360,7 +379,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       Q8Cursor nxt = cur;
       q8_next(sc, nxt);
       // K: row ct of the operand is key k_row
-      if (!wait_or_abort(sm, &sm->kin_full, u & 1)) break;
+      if (!q8_wait(&sm->abort_flag, &sm->kin_full, u & 1)) break;
       ++k_got;
       uint4 in[8];
 #pragma unroll
@@ -370,11 +389,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       fence_proxy_async_smem();
       mbar_arrive(&sm->kin_read);
       if (ct == 0 && nxt.left > 0) {
-        if (!wait_or_abort(sm, &sm->kin_read, u & 1)) break;
+        if (!q8_wait(&sm->abort_flag, &sm->kin_read, u & 1)) break;
         request(nxt, &tmap_k, sm->k_in, &sm->kin_full);
         ++k_asked;
       }
-      if (u > 0 && !wait_or_abort(sm, &sm->k_free, (u - 1) & 1)) break;
+      if (u > 0 && !q8_wait(&sm->abort_flag, &sm->k_free, (u - 1) & 1)) break;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         uint4 h0, h1;
@@ -389,7 +408,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       fence_proxy_async_smem();
       mbar_arrive(&sm->k_full);
       // V: 8 keys x 16 dims, transposed
-      if (!wait_or_abort(sm, &sm->vin_full, u & 1)) break;
+      if (!q8_wait(&sm->abort_flag, &sm->vin_full, u & 1)) break;
       ++v_got;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -399,11 +418,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       fence_proxy_async_smem();
       mbar_arrive(&sm->vin_read);
       if (ct == 0 && nxt.left > 0) {
-        if (!wait_or_abort(sm, &sm->vin_read, u & 1)) break;
+        if (!q8_wait(&sm->abort_flag, &sm->vin_read, u & 1)) break;
         request(nxt, &tmap_v, sm->v_in, &sm->vin_full);
         ++v_asked;
       }
-      if (u > 0 && !wait_or_abort(sm, &sm->v_free, (u - 1) & 1)) break;
+      if (u > 0 && !q8_wait(&sm->abort_flag, &sm->v_free, (u - 1) & 1)) break;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         auto word = [&](const uint4& y) { return w == 0 ? y.x : w == 1 ? y.y : w == 2 ? y.z : y.w; };
@@ -435,21 +454,19 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     int pairs = 0;
     // S of tile x = Q K^T for unit u; `start`: the first of a pair
     auto qk = [&](int x, int u, bool start) {
-      if (!ok) return;
-      if (x == 0) ok = wait_or_abort(sm, &sm->k_full, u & 1);
-      if (ok && start) ok = wait_or_abort(sm, &sm->q_full[x], pairs & 1);
+      if (x == 0) ok = q8_wait(&sm->abort_flag, &sm->k_full, u & 1);
+      if (ok && start) ok = q8_wait(&sm->abort_flag, &sm->q_full[x], pairs & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
       if (lane == 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int lo = 0; lo < 2; ++lo) {
-            const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
-            mma_f16(tmem + 128 * x, sw128_desc(s_q + (2 * x + lo) * 2 * kHalf + off),
-                    sw128_desc(s_k + off), kIdesc, j > 0 || lo > 0 ? 1u : 0u);
-          }
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
+          const uint64_t dk = sw128_desc(s_k + off), dq = sw128_desc(s_q + 4 * x * kHalf + off);
+          mma_f16(tmem + 128 * x, dq, dk, kIdesc, j > 0 ? 1u : 0u);
+          mma_f16(tmem + 128 * x, dq + (2 * kHalf >> 4), dk, kIdesc, 1u);
+        }
         mma_commit(&sm->s_full[x]);
         if (x == 1) mma_commit(&sm->k_free);
       }
@@ -457,43 +474,45 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     };
     // O of tile x += P V
     auto pv = [&](int x, int u, bool start) {
-      if (!ok) return;
-      if (x == 0) ok = wait_or_abort(sm, &sm->v_full, u & 1);
-      if (ok) ok = wait_or_abort(sm, &sm->p_full[x], u & 1);
+      if (x == 0) ok = q8_wait(&sm->abort_flag, &sm->v_full, u & 1);
+      if (ok) ok = q8_wait(&sm->abort_flag, &sm->p_full[x], u & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
       if (lane == 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int lo = 0; lo < 2; ++lo) {
-            const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
-            mma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 16 * j + 8 * lo, sw128_desc(s_v + off),
-                       !start || j > 0 || lo > 0 ? 1u : 0u);
-          }
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t dv = sw128_desc(s_v + (j >> 2) * kHalf + (j & 3) * 32);
+          const uint32_t t_o = tmem + 256 + 128 * x, t_p = tmem + 128 * x + 16 * j;
+          mma_f16_ts(t_o, t_p, dv, !start || j > 0 ? 1u : 0u);
+          mma_f16_ts(t_o, t_p + 8, dv, 1u);
+        }
         mma_commit(&sm->o_full[x]);
         if (x == 1) mma_commit(&sm->v_free);
       }
       __syncwarp();
     };
-    qk(0, 0, true);
-    qk(1, 0, true);
-    bool start = true;
-    for (int u = 0; cur.left > 0 && ok; ++u) {
-      const bool pair_ends = cur.unit + 1 == cur.units;
-      q8_next(sc, cur);
-      const bool more = cur.left > 0;
-      pv(0, u, start);
-      if (more && !pair_ends) qk(0, u + 1, false);
-      pv(1, u, start);
-      if (more && !pair_ends) qk(1, u + 1, false);
-      if (more && pair_ends) {
-        ++pairs;
-        qk(0, u + 1, true);
-        qk(1, u + 1, true);
+    // u = -1: the first unit's scores. Inside a pair PV_A QK_A PV_B QK_B, at its end both PV
+    // before the next pair's scores, which wait for its query rows.
+    bool first = true, pair_ends = true, more = true;
+    for (int u = -1; more && ok; ++u) {
+      if (u >= 0) {
+        pair_ends = cur.unit + 1 == cur.units;
+        q8_next(sc, cur);
+        more = cur.left > 0;
+        if (more && pair_ends) ++pairs;
       }
-      start = pair_ends;
+#pragma unroll 1
+      for (int i = 0; i < 4 && ok; ++i) {
+        const bool is_qk = pair_ends ? i >= 2 : i & 1;
+        const int x = pair_ends ? i & 1 : i >> 1;
+        if (is_qk) {
+          if (more) qk(x, u + 1, pair_ends);
+        } else if (u >= 0) {
+          pv(x, u, first);
+        }
+      }
+      first = pair_ends;
     }
     if (lane == 0) mma_commit(&sm->drain);
     __syncwarp();

@@ -250,6 +250,27 @@ inline bool q8_map(CUtensorMap* map, const int8_t* codes, const Q8Cache& c, int 
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Bounded wait on an mbarrier phase that leaves the issue slots to the warps that work: each
+// try sleeps up to 20 us, the whole wait up to half a second. Gives up (and raises the abort flag
+// and the device error word) at the bound, or once another role has.
+OBN_DEVINL bool q8_wait(volatile int* abort_flag, uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 15); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+  }
+  record_error(DEVERR_MBAR_TIMEOUT);
+  *abort_flag = 1;
+  return false;
+}
+
 // Workspace of a pass of `rows` rows per tile: for each of 2 C slots the sums [rows][128],
 // then the maxima and totals [rows] (all f32).
 OBN_DEVINL float* q8_part_o(float* ws, int rows, int slot) {
