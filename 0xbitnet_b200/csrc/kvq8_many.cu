@@ -61,14 +61,35 @@ static_assert(sizeof(ManySmem) <= 227 * 1024, "shared memory");
 constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(128 >> 3) << 17) |
                             (static_cast<uint32_t>(128 >> 4) << 24);  // f32 = f16 x f16, 128 x 128
 
-// A from tensor memory.
-OBN_DEVINL void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t accumulate) {
+// One MMA, issued by the lane with `one` set while the whole warp runs the same code: operands
+// then stay in uniform registers. (512 MMAs of 128 x 128 x 16 back to back: 106 cycles each from
+// one thread in a branch, 68 like this with A in shared memory and 93 with A in tensor memory.)
+OBN_DEVINL void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t accumulate,
+                       uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(kIdesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(kIdesc), "r"(accumulate), "r"(one)
       : "memory");
+}
+OBN_DEVINL void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t accumulate,
+                       uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(kIdesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+OBN_DEVINL uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
 }
 
 // The key at position (row of K, k index of V) r of a unit: within a group of 8 keys a the
@@ -447,9 +468,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       if (k_asked > k_got) mbar_wait(&sm->kin_full, (k_asked - 1) & 1);
       if (v_asked > v_got) mbar_wait(&sm->vin_full, (v_asked - 1) & 1);
     }
-  } else {
+  } else if (__shfl_sync(0xffffffffu, warp, 0) == 12) {  // uniform to the compiler too
     // ---- MMAs ----------------------------------------------------------------------------------
-    const uint32_t s_q = smem_u32(sm->q[0][0]), s_k = smem_u32(sm->k), s_v = smem_u32(sm->v);
+    const uint32_t one = elect_one(), t_mem = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t d_q = sw128_desc(smem_u32(sm->q[0][0])), d_k = sw128_desc(smem_u32(sm->k)),
+                   d_v = sw128_desc(smem_u32(sm->v));
     bool ok = true;
     int pairs = 0;
     // S of tile x = Q K^T for unit u; `start`: the first of a pair
@@ -459,14 +482,14 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
-      if (lane == 0) {
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t off = (j >> 2) * kHalf + (j & 3) * 32;
-          const uint64_t dk = sw128_desc(s_k + off), dq = sw128_desc(s_q + 4 * x * kHalf + off);
-          mma_f16(tmem + 128 * x, dq, dk, kIdesc, j > 0 ? 1u : 0u);
-          mma_f16(tmem + 128 * x, dq + (2 * kHalf >> 4), dk, kIdesc, 1u);
-        }
+      const uint64_t q0 = d_q + x * (4 * kHalf >> 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t off = ((j >> 2) * kHalf + (j & 3) * 32) >> 4;
+        mma_ss(t_mem + 128 * x, q0 + off, d_k + off, j > 0 ? 1u : 0u, one);
+        mma_ss(t_mem + 128 * x, q0 + off + (2 * kHalf >> 4), d_k + off, 1u, one);
+      }
+      if (one) {
         mma_commit(&sm->s_full[x]);
         if (x == 1) mma_commit(&sm->k_free);
       }
@@ -479,14 +502,14 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
-      if (lane == 0) {
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          const uint64_t dv = sw128_desc(s_v + (j >> 2) * kHalf + (j & 3) * 32);
-          const uint32_t t_o = tmem + 256 + 128 * x, t_p = tmem + 128 * x + 16 * j;
-          mma_f16_ts(t_o, t_p, dv, !start || j > 0 ? 1u : 0u);
-          mma_f16_ts(t_o, t_p + 8, dv, 1u);
-        }
+      const uint32_t t_o = t_mem + 256 + 128 * x, t_p = t_mem + 128 * x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t off = ((j >> 2) * kHalf + (j & 3) * 32) >> 4;
+        mma_ts(t_o, t_p + 16 * j, d_v + off, !start || j > 0 ? 1u : 0u, one);
+        mma_ts(t_o, t_p + 16 * j + 8, d_v + off, 1u, one);
+      }
+      if (one) {
         mma_commit(&sm->o_full[x]);
         if (x == 1) mma_commit(&sm->v_free);
       }
@@ -514,7 +537,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       }
       first = pair_ends;
     }
-    if (lane == 0) mma_commit(&sm->drain);
+    if (one) mma_commit(&sm->drain);
     __syncwarp();
     mbar_wait(&sm->drain, 0);
     __syncwarp();
