@@ -8,14 +8,15 @@
 //
 // One CTA per SM works on a pair of tiles, 2 x 128 query rows (token, group head) of a sequence
 // and KV head, so every converted key block serves 256 rows, and on units of 128 keys
-// (kvq8_sched.cuh). Roles, 13 warps:
-//   warps 0-3, 4-7  softmax of tile A, B: a thread is a row. S from tensor memory twice (maximum;
-//                   weights), the weights back over S as the A operand of the second product.
-//   warps 8-11      codes to f16: TMA staging -> registers -> shared memory in the MMA's layout;
-//                   V is transposed on the way. The staging is requested again as soon as
-//                   it is read.
-//   warp 12         issues the MMAs, in the order  PV_A(u) QK_A(u+1) PV_B(u) QK_B(u+1): while
-//                   one tile's softmax runs, the other tile's products do.
+// (kvq8_sched.cuh). Roles, 21 warps:
+//   warps 0-7, 8-15  softmax of tile A, B: two threads a row, 64 keys (and 64 dims of O) each. S
+//                    from tensor memory twice (maximum; weights), the weights back over S as the
+//                    A operand of the second product.
+//   warps 16-19      codes to f16: TMA staging -> registers -> shared memory in the MMA's layout;
+//                    V is transposed on the way. The staging is requested again as soon as
+//                    it is read.
+//   warp 20          issues the MMAs, in the order  PV_A(u) QK_A(u+1) PV_B(u) QK_B(u+1): while
+//                    one tile's softmax runs, the other tile's products do.
 // Tensor memory: S (and P) of A and B, 2 x 128 columns, O of A and B, 2 x 128.
 //
 // Softmax. With s = q.k, f = scale of q, key block and log2 e, v's block scale 2^lv: a weight
@@ -23,6 +24,8 @@
 // whatever the scales of other blocks, and O adds w times codes. R moves only when a row's
 // maximum of s f + lv exceeds it by 15 (w <= 2^15 fits f16); then O is rescaled in
 // tensor memory. The total is the sum of w 2^(lv0 - lv), exact factors, lv0 fixed for a part.
+// The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
+// unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -39,7 +42,8 @@ namespace {
 
 constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
-constexpr int kThreads = 416;
+constexpr int kThreads = 672;
+constexpr int kDrain = 4;
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
 
@@ -51,6 +55,8 @@ struct ManySmem {
   uint64_t kin_full, vin_full, kin_read, vin_read;
   uint64_t k_full, k_free, v_full, v_free;
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t swap[2][4];         // two threads of a row exchange a value
+  float swapped[2][2][128];    // [tile][half][row]
   uint64_t drain;
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -137,16 +143,17 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     mbar_init(&sm->v_full, 128);
     mbar_init(&sm->v_free, 1);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sm->q_full[x], 128);
+      mbar_init(&sm->q_full[x], 256);
       mbar_init(&sm->s_full[x], 1);
-      mbar_init(&sm->p_full[x], 128);
+      mbar_init(&sm->p_full[x], 256);
       mbar_init(&sm->o_full[x], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&sm->swap[x][i], 64);
     }
     mbar_init(&sm->drain, 1);
     sm->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(&sm->tmem_base, 512);
     tmem_relinquish();
   }
@@ -160,13 +167,19 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
 
   if (cur.left == 0) {
     // nothing for this CTA
-  } else if (warp < 8) {
-    // ---- softmax: thread = row `row` of tile x ------------------------------------------
-    const int x = warp >> 2, row = tid & 127;
+  } else if (warp < 16) {
+    // ---- softmax: thread = half hf of row `row` of tile x ---------------------------------
+    const int x = warp >> 3, hf = (warp >> 2) & 1, row = tid & 127;
     const int H = sc.G * sc.Hkv, rows_seq = sc.n * sc.G;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_base + 128 * x, t_o = tmem + lane_base + 256 + 128 * x;
-    float R = -INFINITY, l = 0.0f, lv0 = 0.0f, sq = 0.0f, scl = 0.0f;
+    const uint32_t t_s = tmem + lane_base + 128 * x + 64 * hf,
+                   t_o = tmem + lane_base + 256 + 128 * x + 64 * hf;
+    // the copy of O: [4 dims] of this half, row by row
+    float4* copy = reinterpret_cast<float4*>(ws + q8_workspace(kRows, kManyMaxCtas) / sizeof(float)) +
+                   ((static_cast<size_t>(blockIdx.x) * 2 + x) * 2 + hf) * (16 * 128) + row;
+    float R = -INFINITY, l = 0.0f, lv0 = 0.0f, sq = 0.0f, scl = 0.0f, copy_R = 0.0f;
+    int part_u = 0;  // units of the part so far
+    uint32_t swaps = 0;
     int lim = 0, u_first = 0, r = 0;
     size_t row_off = 0;  // of this row in q and out, in floats
     bool fresh = true, ok = true;
@@ -177,6 +190,16 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
                  ? __ldg((lane < 8 ? k_scale : v_scale) +
                          (static_cast<size_t>(c.b) * nblk + blk) * sc.Hkv + c.kvh)
                  : 0.0f;
+    };
+    // this half's value to the other one's thread, and back; false after an abort
+    auto exchange = [&](float mine, float* other) {
+      sm->swapped[x][hf][row] = mine;
+      mbar_arrive(&sm->swap[x][warp & 3]);
+      const bool came =
+          __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->swap[x][warp & 3], swaps & 1));
+      ++swaps;
+      *other = sm->swapped[x][hf ^ 1][row];
+      return came;
     };
     scl = load_scale(cur);
     for (int u = 0; cur.left > 0; ++u) {
@@ -205,8 +228,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         sq = (bad ? __int_as_float(0x7FC00000) : __int_as_float((127 + ex - 14) << 23)) * scale_log2;
         uint8_t* hi = sm->q[x][0] + row * 128;
         uint8_t* lo = sm->q[x][1] + row * 128;
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
+#pragma unroll 2
+        for (int i = hf * (D / 16); i < (hf + 1) * (D / 16); ++i) {
           float e[8] = {};
           if (real && !bad) {
             const float4 a = __ldg(src + 2 * i), b = __ldg(src + 2 * i + 1);
@@ -233,6 +256,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         lim = real ? min(cur.len, q8_limit(sc, cur.len, r)) : 0;
         R = -INFINITY;
         l = 0.0f;
+        part_u = 0;
         // the reference of the value scales: the unit's largest exponent
         float top = lane >= 8 && lane < 16 && scl > 0.0f ? scl : 0.0f;
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
@@ -253,23 +277,24 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->s_full[x], u & 1));
       if (!ok) break;
       tc_fence_after();
-      // 1. the largest s f + lv. The loops over 16-key blocks stay loops: unrolled, the two softmax
-      // groups, the converters and the MMA warp evict each other's instructions (both passes
-      // unrolled fully: 8600 cycles a unit; in halves: 5600).
+      // 1. the largest s f + lv of the row. The loops over 16-key blocks stay loops: unrolled, the
+      // softmax warps, the converters and the MMA warp evict each other's instructions (both
+      // passes unrolled: 8600 cycles a unit; in halves: 5600).
       float xr = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t s[32];
         tmem_ld32(t_s + 32 * c, s);
-        const float f0 = sq * __shfl_sync(0xffffffffu, scl_now, 2 * c);
-        const float f1 = sq * __shfl_sync(0xffffffffu, scl_now, 2 * c + 1);
-        const float lv_0 = __shfl_sync(0xffffffffu, lv_lane, 8 + 2 * c);
-        const float lv_1 = __shfl_sync(0xffffffffu, lv_lane, 9 + 2 * c);
+        const int b = 4 * hf + 2 * c;  // 16-key block
+        const float f0 = sq * __shfl_sync(0xffffffffu, scl_now, b);
+        const float f1 = sq * __shfl_sync(0xffffffffu, scl_now, b + 1);
+        const float lv_0 = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
+        const float lv_1 = __shfl_sync(0xffffffffu, lv_lane, 9 + b);
         tmem_ld_wait();
         if (!all) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (32 * c + key_in_32(i, c) >= seen) s[i] = 0xFF800000u;  // -inf
+            if (16 * b + key_in_32(i, b >> 1) >= seen) s[i] = 0xFF800000u;  // -inf
         }
         float m[4];
 #pragma unroll
@@ -282,35 +307,56 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         xr = fmaxf(xr, m0 == -INFINITY ? -INFINITY : fmaf(m0, f0, lv_0));
         xr = fmaxf(xr, m1 == -INFINITY ? -INFINITY : fmaf(m1, f1, lv_1));
       }
+      float xo;
+      if (!exchange(xr, &xo)) break;
+      xr = fmaxf(xr, xo);
       const bool grow = xr > R + 15.0f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float Rn = grow ? ceilf(xr) - 7.0f : R;
-        const float corr = grow ? ex2(R - Rn) : 1.0f;
-        l *= corr;
-        R = Rn;
-        if (!fresh) {  // O holds sums of this part
-          ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
-          if (!ok) break;
-          tc_fence_after();
+      const float Rn = grow ? ceilf(xr) - 7.0f : R;
+      const float corr = grow ? ex2(R - Rn) : 1.0f;
+      const bool drain = part_u > 0 && part_u % kDrain == 0;
+      l *= corr;
+      if (part_u > 0 && (drain || __any_sync(0xffffffffu, grow))) {
+        ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const float old = part_u == kDrain ? 0.0f : copy_R == R ? 1.0f : ex2(copy_R - R);
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * c, o);
-            tmem_ld_wait();
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_o + 16 * c, o);
+          tmem_ld_wait();
+          if (drain) {  // to the copy, at the reference R
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st32(t_o + 32 * c, o);
+            for (int i = 0; i < 4; ++i) {
+              float4* at = copy + (4 * c + i) * 128;
+              float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (part_u > kDrain) y = *at;
+              y.x = fmaf(y.x, old, __uint_as_float(o[4 * i]));
+              y.y = fmaf(y.y, old, __uint_as_float(o[4 * i + 1]));
+              y.z = fmaf(y.z, old, __uint_as_float(o[4 * i + 2]));
+              y.w = fmaf(y.w, old, __uint_as_float(o[4 * i + 3]));
+              *at = y;
+            }
+          } else {  // to the new reference
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(t_o + 16 * c, o);
           }
-          tmem_st_wait();
         }
+        if (drain)
+          copy_R = R;
+        else
+          tmem_st_wait();
       }
+      R = Rn;
+      ++part_u;
       fresh = false;
       // 2. the weights, over the scores: 8 columns of high and 8 of low halves per 16 keys
       const float Rs = R == -INFINITY ? 0.0f : R;
 #pragma unroll 1
-      for (int b = 0; b < 8; ++b) {
+      for (int b = 4 * hf; b < 4 * hf + 4; ++b) {
         uint32_t s[16];
-        tmem_ld16(t_s + 16 * b, s);
+        tmem_ld16(t_s + 16 * (b & 3), s);
         const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
         const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
         const float poison = __shfl_sync(0xffffffffu, bad_lane, 8 + b);
@@ -337,12 +383,12 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
-          const float2 hf = __half22float2(h);
-          const __half2 m = __floats2half2_rn(w[2 * i] - hf.x, w[2 * i + 1] - hf.y);
+          const float2 hf2 = __half22float2(h);
+          const __half2 m = __floats2half2_rn(w[2 * i] - hf2.x, w[2 * i + 1] - hf2.y);
           s[i] = *reinterpret_cast<const uint32_t*>(&h);
           s[8 + i] = *reinterpret_cast<const uint32_t*>(&m);
         }
-        tmem_st16(t_s + 16 * b, s);
+        tmem_st16(t_s + 16 * (b & 3), s);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -353,26 +399,38 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], u & 1));
         if (!ok) break;
         tc_fence_after();
+        float lo;
+        if (!exchange(l, &lo)) break;
+        l = hf ? lo + l : l + lo;
         const bool whole = pair_ends && u_first == 0;
         const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
         const float unit = ex2(lv0) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
-        float* dst = whole ? out + row_off : q8_part_o(ws, kRows, slot) + (128 * x + row) * D;
-        if (!whole) {
+        float* dst = (whole ? out + row_off : q8_part_o(ws, kRows, slot) + (128 * x + row) * D) + 64 * hf;
+        if (!whole && hf == 0) {
           float* ml = q8_part_ml(ws, kRows, slot);
           ml[128 * x + row] = R == -INFINITY ? -INFINITY : R - lv0;
           ml[kRows + 128 * x + row] = l;
         }
+        const bool copied = part_u > kDrain;
+        const float old = copy_R == R ? 1.0f : ex2(copy_R - R);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * c, o);
+          uint32_t o[16];
+          tmem_ld16(t_o + 16 * c, o);
           tmem_ld_wait();
           if (r < rows_seq) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4*>(dst + 32 * c + 4 * i) =
-                  make_float4(__uint_as_float(o[4 * i]) * unit, __uint_as_float(o[4 * i + 1]) * unit,
-                              __uint_as_float(o[4 * i + 2]) * unit, __uint_as_float(o[4 * i + 3]) * unit);
+            for (int i = 0; i < 4; ++i) {
+              float4 y = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              if (copied) {
+                const float4 z = copy[(4 * c + i) * 128];
+                y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z),
+                                fmaf(z.w, old, y.w));
+              }
+              *reinterpret_cast<float4*>(dst + 16 * c + 4 * i) =
+                  make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
+            }
           }
         }
         tc_fence_before();
@@ -380,9 +438,9 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       }
       cur = nxt;
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ---- codes to f16 ------------------------------------------------------------------------
-    const int ct = tid - 256, cw = ct >> 5;
+    const int ct = tid - 512, cw = ct >> 5;
     auto request = [&](const Q8Cursor& c, const CUtensorMap* map, uint8_t* dst, uint64_t* bar) {
       const int k0 = c.unit * kUnitKeys;
       mbar_arrive_expect_tx(bar, kUnitKeys * D);
@@ -468,7 +526,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       if (k_asked > k_got) mbar_wait(&sm->kin_full, (k_asked - 1) & 1);
       if (v_asked > v_got) mbar_wait(&sm->vin_full, (v_asked - 1) & 1);
     }
-  } else if (__shfl_sync(0xffffffffu, warp, 0) == 12) {  // uniform to the compiler too
+  } else if (__shfl_sync(0xffffffffu, warp, 0) == 20) {  // uniform to the compiler too
     // ---- MMAs ----------------------------------------------------------------------------------
     const uint32_t one = elect_one(), t_mem = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t d_q = sw128_desc(smem_u32(sm->q[0][0])), d_k = sw128_desc(smem_u32(sm->k)),
@@ -517,7 +575,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     };
     // u = -1: the first unit's scores. Inside a pair PV_A QK_A PV_B QK_B, at its end both PV
     // before the next pair's scores, which wait for its query rows.
-    bool first = true, pair_ends = true, more = true;
+    bool pair_ends = true, more = true;
+    int part_u = 0;  // units of the part so far: O starts anew every kDrain of them
     for (int u = -1; more && ok; ++u) {
       if (u >= 0) {
         pair_ends = cur.unit + 1 == cur.units;
@@ -532,10 +591,10 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         if (is_qk) {
           if (more) qk(x, u + 1, pair_ends);
         } else if (u >= 0) {
-          pv(x, u, first);
+          pv(x, u, part_u % kDrain == 0);
         }
       }
-      first = pair_ends;
+      if (u >= 0) part_u = pair_ends ? 0 : part_u + 1;
     }
     if (one) mma_commit(&sm->drain);
     __syncwarp();
@@ -545,7 +604,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 20) tmem_dealloc(tmem, 512);
 }
 
 // k_q8_join for tiles of many rows: a warp per row, few parts each.
@@ -600,7 +659,10 @@ __global__ __launch_bounds__(256) void k_q8_join_rows(Q8Sched sc, float* __restr
 
 }  // namespace
 
-size_t attention_q8_many_workspace_bytes() { return q8_workspace(kRows, kManyMaxCtas); }
+size_t attention_q8_many_workspace_bytes() {
+  return q8_workspace(kRows, kManyMaxCtas) +
+         static_cast<size_t>(kManyMaxCtas) * kRows * D * sizeof(float);  // copies of O
+}
 
 cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, int H, int seq_len,
                                      const int* lens_dev, float scale_log2, float* out, void* ws,

@@ -279,7 +279,7 @@ OBN_DEVINL float* q8_part_o(float* ws, int rows, int slot) {
 OBN_DEVINL float* q8_part_ml(float* ws, int rows, int slot) {
   return q8_part_o(ws, rows, slot) + static_cast<size_t>(rows) * kQ8HeadDim;
 }
-inline size_t q8_workspace(int rows, int ctas) {
+constexpr size_t q8_workspace(int rows, int ctas) {
   return static_cast<size_t>(2) * ctas * rows * (kQ8HeadDim + 2) * sizeof(float);
 }
 
