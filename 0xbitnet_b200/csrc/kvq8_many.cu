@@ -44,6 +44,7 @@ constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
 constexpr int kDrain = 4;
+constexpr int kBadRow = 0x7FFF;  // exponent of a row of q that is not finite
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
 
@@ -57,6 +58,8 @@ struct ManySmem {
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint64_t swap[2][4];         // two threads of a row exchange a value
   float swapped[2][2][128];    // [tile][half][row]
+  int16_t q_exp[2][128];       // rows of q are scaled by 2^(14 - exponent)
+  uint64_t staged[2];          // rows of O on their way out
   uint64_t drain;
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -147,6 +150,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       mbar_init(&sm->s_full[x], 1);
       mbar_init(&sm->p_full[x], 256);
       mbar_init(&sm->o_full[x], 1);
+      mbar_init(&sm->staged[x], 256);
       for (int i = 0; i < 4; ++i) mbar_init(&sm->swap[x][i], 64);
     }
     mbar_init(&sm->drain, 1);
@@ -179,9 +183,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
                    ((static_cast<size_t>(blockIdx.x) * 2 + x) * 2 + hf) * (16 * 128) + row;
     float R = -INFINITY, l = 0.0f, lv0 = 0.0f, sq = 0.0f, scl = 0.0f, copy_R = 0.0f;
     int part_u = 0;  // units of the part so far
-    uint32_t swaps = 0;
-    int lim = 0, u_first = 0, r = 0;
-    size_t row_off = 0;  // of this row in q and out, in floats
+    uint32_t swaps = 0, stagings = 0;
+    int lim = 0, u_first = 0, r = 0, pairs = 0;
     bool fresh = true, ok = true;
     // lanes 0-7: the unit's key scales, 8-15: its value scales
     auto load_scale = [&](const Q8Cursor& c) {
@@ -206,53 +209,63 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       const int k0 = cur.unit * kUnitKeys;
       Q8Cursor nxt = cur;
       q8_next(sc, nxt);
-      if (fresh) {  // this row of q as f16 hi and lo, scaled to below 2^14
+      if (fresh) {  // 16 rows of q a warp, as f16 hi and lo scaled to below 2^14
         u_first = cur.unit;
-        r = cur.tile * kRows + 128 * x + row;
-        const bool real = r < rows_seq;
-        const int t = real ? r / sc.G : 0, g = real ? r - t * sc.G : 0;
-        row_off = ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D;
-        const float4* src = reinterpret_cast<const float4*>(q + row_off);
-        uint32_t big = 0;
-        if (real) {
-#pragma unroll 8
-          for (int i = 0; i < D / 4; ++i) {
-            const float4 y = __ldg(src + i);
-            big = max(big, max(max(__float_as_uint(y.x) & 0x7FFFFFFFu, __float_as_uint(y.y) & 0x7FFFFFFFu),
-                               max(__float_as_uint(y.z) & 0x7FFFFFFFu, __float_as_uint(y.w) & 0x7FFFFFFFu)));
-          }
-        }
-        const bool bad = big >= 0x7F800000u;
-        const int ex = max(static_cast<int>(big >> 23) - 126, -90);  // |q| < 2^ex
-        const float up = __int_as_float((127 + 14 - ex) << 23);
-        sq = (bad ? __int_as_float(0x7FC00000) : __int_as_float((127 + ex - 14) << 23)) * scale_log2;
-        uint8_t* hi = sm->q[x][0] + row * 128;
-        uint8_t* lo = sm->q[x][1] + row * 128;
-#pragma unroll 2
-        for (int i = hf * (D / 16); i < (hf + 1) * (D / 16); ++i) {
-          float e[8] = {};
-          if (real && !bad) {
-            const float4 a = __ldg(src + 2 * i), b = __ldg(src + 2 * i + 1);
-            e[0] = a.x * up, e[1] = a.y * up, e[2] = a.z * up, e[3] = a.w * up;
-            e[4] = b.x * up, e[5] = b.y * up, e[6] = b.z * up, e[7] = b.w * up;
-          }
-          uint4 wh, wl;
-          uint32_t* ph = &wh.x;
-          uint32_t* pl = &wl.x;
+        const int w = warp & 7;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16; i0 += 4) {
+          float4 y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
-            const float2 hf = __half22float2(h);
-            const __half2 m = __floats2half2_rn(e[2 * j] - hf.x, e[2 * j + 1] - hf.y);
-            ph[j] = *reinterpret_cast<const uint32_t*>(&h);
-            pl[j] = *reinterpret_cast<const uint32_t*>(&m);
+          for (int i = 0; i < 4; ++i) {
+            const int qr = cur.tile * kRows + 128 * x + 16 * w + i0 + i;
+            const int t = qr / sc.G, g = qr - t * sc.G;
+            y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (qr < rows_seq)
+              y[i] = __ldg(reinterpret_cast<const float4*>(
+                  q + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D + 4 * lane));
           }
-          const int at = (i >> 3) * kHalf + (((i & 7) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(hi + at) = wh;
-          *reinterpret_cast<uint4*>(lo + at) = wl;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int qrow = 16 * w + i0 + i;
+            // the largest magnitude's bits: an infinity or NaN shows as exponent 255
+            const uint32_t big = __reduce_max_sync(
+                0xffffffffu,
+                max(max(__float_as_uint(y[i].x) & 0x7FFFFFFFu, __float_as_uint(y[i].y) & 0x7FFFFFFFu),
+                    max(__float_as_uint(y[i].z) & 0x7FFFFFFFu, __float_as_uint(y[i].w) & 0x7FFFFFFFu)));
+            const bool bad = big >= 0x7F800000u;
+            const int ex = max(static_cast<int>(big >> 23) - 126, -90);  // |q| < 2^ex
+            const float up = __int_as_float((127 + 14 - ex) << 23);
+            if (lane == 0) sm->q_exp[x][qrow] = static_cast<int16_t>(bad ? kBadRow : ex);
+            uint2 wh = make_uint2(0u, 0u), wl = make_uint2(0u, 0u);
+            if (!bad) {
+              const float e[4] = {y[i].x * up, y[i].y * up, y[i].z * up, y[i].w * up};
+              uint32_t* ph = &wh.x;
+              uint32_t* pl = &wl.x;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
+                const float2 back = __half22float2(h);
+                const __half2 m = __floats2half2_rn(e[2 * j] - back.x, e[2 * j + 1] - back.y);
+                ph[j] = *reinterpret_cast<const uint32_t*>(&h);
+                pl[j] = *reinterpret_cast<const uint32_t*>(&m);
+              }
+            }
+            // 8 bytes of 16-byte chunk (lane / 2) % 8 of the half lane / 16
+            const int at = (lane >> 4) * kHalf + qrow * 128 +
+                           ((((lane >> 1) & 7) ^ (qrow & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(sm->q[x][0] + at) = wh;
+            *reinterpret_cast<uint2*>(sm->q[x][1] + at) = wl;
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(&sm->q_full[x]);
+        ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->q_full[x], pairs & 1));
+        if (!ok) break;
+        ++pairs;
+        const int qe = sm->q_exp[x][row];
+        sq = (qe == kBadRow ? __int_as_float(0x7FC00000) : __int_as_float((127 + qe - 14) << 23)) * scale_log2;
+        r = cur.tile * kRows + 128 * x + row;
+        const bool real = r < rows_seq;
         lim = real ? min(cur.len, q8_limit(sc, cur.len, r)) : 0;
         R = -INFINITY;
         l = 0.0f;
@@ -319,23 +332,34 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
         if (!ok) break;
         tc_fence_after();
-        const float old = part_u == kDrain ? 0.0f : copy_R == R ? 1.0f : ex2(copy_R - R);
+        // the copy keeps its reference while O's is within 2^60 of it
+        const bool begin = part_u == kDrain || copy_R == -INFINITY;
+        const bool shift = drain && !begin && R > copy_R + 60.0f;
+        const float to_copy = begin || shift ? 1.0f : ex2(R - copy_R);
+        const float old = shift ? ex2(copy_R - R) : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[16];
           tmem_ld16(t_o + 16 * c, o);
           tmem_ld_wait();
-          if (drain) {  // to the copy, at the reference R
+          if (drain) {  // to the copy
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float4* at = copy + (4 * c + i) * 128;
-              float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if (part_u > kDrain) y = *at;
-              y.x = fmaf(y.x, old, __uint_as_float(o[4 * i]));
-              y.y = fmaf(y.y, old, __uint_as_float(o[4 * i + 1]));
-              y.z = fmaf(y.z, old, __uint_as_float(o[4 * i + 2]));
-              y.w = fmaf(y.w, old, __uint_as_float(o[4 * i + 3]));
-              *at = y;
+              float4 y = make_float4(__uint_as_float(o[4 * i]) * to_copy, __uint_as_float(o[4 * i + 1]) * to_copy,
+                                     __uint_as_float(o[4 * i + 2]) * to_copy, __uint_as_float(o[4 * i + 3]) * to_copy);
+              if (begin || shift) {
+                if (shift) {
+                  const float4 z = __ldcg(at);
+                  y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z),
+                                  fmaf(z.w, old, y.w));
+                }
+                __stcg(at, y);
+              } else {  // nothing to wait for
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at),
+                             "f"(y.x), "f"(y.y), "f"(y.z), "f"(y.w)
+                             : "memory");
+              }
             }
           } else {  // to the new reference
 #pragma unroll
@@ -343,10 +367,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
             tmem_st16(t_o + 16 * c, o);
           }
         }
-        if (drain)
-          copy_R = R;
-        else
+        if (drain) {
+          if (begin || shift) copy_R = R;
+        } else {
           tmem_st_wait();
+        }
       }
       R = Rn;
       ++part_u;
@@ -405,7 +430,6 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         const bool whole = pair_ends && u_first == 0;
         const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
         const float unit = ex2(lv0) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
-        float* dst = (whole ? out + row_off : q8_part_o(ws, kRows, slot) + (128 * x + row) * D) + 64 * hf;
         if (!whole && hf == 0) {
           float* ml = q8_part_ml(ws, kRows, slot);
           ml[128 * x + row] = R == -INFINITY ? -INFINITY : R - lv0;
@@ -413,26 +437,49 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         }
         const bool copied = part_u > kDrain;
         const float old = copy_R == R ? 1.0f : ex2(copy_R - R);
+        // through the query rows' shared memory (nobody needs them any more), so that rows go
+        // out whole: [row][dim], 16-byte pieces swizzled
+        float* stage = reinterpret_cast<float*>(sm->q[x][0]);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[16];
           tmem_ld16(t_o + 16 * c, o);
-          tmem_ld_wait();
-          if (r < rows_seq) {
+          float4 z[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float4 y = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-              if (copied) {
-                const float4 z = copy[(4 * c + i) * 128];
-                y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z),
-                                fmaf(z.w, old, y.w));
-              }
-              *reinterpret_cast<float4*>(dst + 16 * c + 4 * i) =
-                  make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
-            }
+          for (int i = 0; i < 4; ++i)
+            z[i] = copied ? __ldcg(copy + (4 * c + i) * 128) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 y = copied ? make_float4(fmaf(z[i].x, old, __uint_as_float(o[4 * i])),
+                                                  fmaf(z[i].y, old, __uint_as_float(o[4 * i + 1])),
+                                                  fmaf(z[i].z, old, __uint_as_float(o[4 * i + 2])),
+                                                  fmaf(z[i].w, old, __uint_as_float(o[4 * i + 3])))
+                                    : make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                  __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            const int piece = 16 * hf + 4 * c + i;
+            *reinterpret_cast<float4*>(stage + row * D + 4 * (piece ^ (row & 31))) =
+                make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
           }
         }
+        mbar_arrive(&sm->staged[x]);
+        ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->staged[x], stagings & 1));
+        ++stagings;
+        if (!ok) break;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int orow = 16 * (warp & 7) + i, qr = cur.tile * kRows + 128 * x + orow;
+          if (qr >= rows_seq) break;
+          const int t = qr / sc.G, g = qr - t * sc.G;
+          float* dst = whole ? out + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D
+                             : q8_part_o(ws, kRows, slot) + (128 * x + orow) * D;
+          *reinterpret_cast<float4*>(dst + 4 * lane) =
+              *reinterpret_cast<const float4*>(stage + orow * D + 4 * (lane ^ (orow & 31)));
+        }
+        mbar_arrive(&sm->staged[x]);  // the stage becomes query rows again
+        ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->staged[x], stagings & 1));
+        ++stagings;
+        if (!ok) break;
         tc_fence_before();
         fresh = true;
       }
