@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -276,12 +277,13 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         lv0 = top > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127) : 0.0f;
       }
       // exponents of the value scales (of zero and poisoned blocks: any, the weights of a zero
-      // one are left out of P and count in the total) and what poisons a total: 0, or NaN
+      // one are left out of P and count in the total)
       const bool plain = scl > 0.0f;
       const float lv_lane =
           plain ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127) : lv0;
-      const float bad_lane = scl - scl;
-      const uint32_t zero = __ballot_sync(0xffffffffu, scl == 0.0f) >> 8;
+      // a block's part of the total counts times this: 2^(lv0 - lv), NaN for a poisoned one
+      const float lf_lane = ex2(fminf(fmaxf(lv0 - lv_lane, -126.0f), 126.0f)) + (scl - scl);
+      const uint32_t zero = (__ballot_sync(0xffffffffu, scl == 0.0f) >> 8) & 255u;
       const float scl_now = scl;
       if (nxt.left > 0) scl = load_scale(nxt);
 
@@ -293,33 +295,42 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       // 1. the largest s f + lv of the row. The loops over 16-key blocks stay loops: unrolled, the
       // softmax warps, the converters and the MMA warp evict each other's instructions (both
       // passes unrolled: 8600 cycles a unit; in halves: 5600).
+      // Units where nothing is masked and no block is zero have code of their own: compiled as
+      // one, the masks cost every element two selects and two compares.
       float xr = -INFINITY;
+      auto largest = [&](auto clean) {
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32];
-        tmem_ld32(t_s + 32 * c, s);
-        const int b = 4 * hf + 2 * c;  // 16-key block
-        const float f0 = sq * __shfl_sync(0xffffffffu, scl_now, b);
-        const float f1 = sq * __shfl_sync(0xffffffffu, scl_now, b + 1);
-        const float lv_0 = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
-        const float lv_1 = __shfl_sync(0xffffffffu, lv_lane, 9 + b);
-        tmem_ld_wait();
-        if (!all) {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          tmem_ld32(t_s + 32 * c, s);
+          const int b = 4 * hf + 2 * c;  // 16-key block
+          const float f0 = sq * __shfl_sync(0xffffffffu, scl_now, b);
+          const float f1 = sq * __shfl_sync(0xffffffffu, scl_now, b + 1);
+          const float lv_0 = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
+          const float lv_1 = __shfl_sync(0xffffffffu, lv_lane, 9 + b);
+          tmem_ld_wait();
+          if constexpr (!decltype(clean)::value) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (16 * b + key_in_32(i, b >> 1) >= seen) s[i] = 0xFF800000u;  // -inf
+            for (int i = 0; i < 32; ++i)
+              if (16 * b + key_in_32(i, b >> 1) >= seen) s[i] = 0xFF800000u;  // -inf
+          }
+          float m[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            m[i] = __uint_as_float(s[8 * i]);
+#pragma unroll
+            for (int j = 1; j < 8; ++j) m[i] = fmaxf(m[i], __uint_as_float(s[8 * i + j]));
+          }
+          const float m0 = fmaxf(m[0], m[1]), m1 = fmaxf(m[2], m[3]);
+          xr = fmaxf(xr, m0 == -INFINITY ? -INFINITY : fmaf(m0, f0, lv_0));
+          xr = fmaxf(xr, m1 == -INFINITY ? -INFINITY : fmaf(m1, f1, lv_1));
         }
-        float m[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = __uint_as_float(s[8 * i]);
-#pragma unroll
-          for (int j = 1; j < 8; ++j) m[i] = fmaxf(m[i], __uint_as_float(s[8 * i + j]));
-        }
-        const float m0 = fmaxf(m[0], m[1]), m1 = fmaxf(m[2], m[3]);
-        xr = fmaxf(xr, m0 == -INFINITY ? -INFINITY : fmaf(m0, f0, lv_0));
-        xr = fmaxf(xr, m1 == -INFINITY ? -INFINITY : fmaf(m1, f1, lv_1));
-      }
+      };
+      const bool is_clean = all && zero == 0;
+      if (is_clean)
+        largest(std::true_type{});
+      else
+        largest(std::false_type{});
       float xo;
       if (!exchange(xr, &xo)) break;
       xr = fmaxf(xr, xo);
@@ -332,34 +343,25 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
         if (!ok) break;
         tc_fence_after();
-        // the copy keeps its reference while O's is within 2^60 of it
-        const bool begin = part_u == kDrain || copy_R == -INFINITY;
-        const bool shift = drain && !begin && R > copy_R + 60.0f;
-        const float to_copy = begin || shift ? 1.0f : ex2(R - copy_R);
-        const float old = shift ? ex2(copy_R - R) : 1.0f;
+        const float old = copy_R == R ? 1.0f : ex2(copy_R - R);
+        const bool add = drain && part_u > kDrain;
+        float4 z[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = add ? __ldcg(copy + i * 128) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[16];
           tmem_ld16(t_o + 16 * c, o);
           tmem_ld_wait();
-          if (drain) {  // to the copy
+          if (drain) {  // to the copy, at the reference R; the next piece of it on its way
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float4* at = copy + (4 * c + i) * 128;
-              float4 y = make_float4(__uint_as_float(o[4 * i]) * to_copy, __uint_as_float(o[4 * i + 1]) * to_copy,
-                                     __uint_as_float(o[4 * i + 2]) * to_copy, __uint_as_float(o[4 * i + 3]) * to_copy);
-              if (begin || shift) {
-                if (shift) {
-                  const float4 z = __ldcg(at);
-                  y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z),
-                                  fmaf(z.w, old, y.w));
-                }
-                __stcg(at, y);
-              } else {  // nothing to wait for
-                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at),
-                             "f"(y.x), "f"(y.y), "f"(y.z), "f"(y.w)
-                             : "memory");
-              }
+              const float4 y = make_float4(fmaf(z[i].x, old, __uint_as_float(o[4 * i])),
+                                           fmaf(z[i].y, old, __uint_as_float(o[4 * i + 1])),
+                                           fmaf(z[i].z, old, __uint_as_float(o[4 * i + 2])),
+                                           fmaf(z[i].w, old, __uint_as_float(o[4 * i + 3])));
+              if (add && c < 3) z[i] = __ldcg(copy + (4 * c + 4 + i) * 128);
+              __stcg(copy + (4 * c + i) * 128, y);
             }
           } else {  // to the new reference
 #pragma unroll
@@ -367,54 +369,59 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
             tmem_st16(t_o + 16 * c, o);
           }
         }
-        if (drain) {
-          if (begin || shift) copy_R = R;
-        } else {
+        if (drain)
+          copy_R = R;
+        else
           tmem_st_wait();
-        }
       }
       R = Rn;
       ++part_u;
       fresh = false;
       // 2. the weights, over the scores: 8 columns of high and 8 of low halves per 16 keys
       const float Rs = R == -INFINITY ? 0.0f : R;
+      auto weights = [&](auto clean) {
 #pragma unroll 1
-      for (int b = 4 * hf; b < 4 * hf + 4; ++b) {
-        uint32_t s[16];
-        tmem_ld16(t_s + 16 * (b & 3), s);
-        const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
-        const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b);
-        const float poison = __shfl_sync(0xffffffffu, bad_lane, 8 + b);
-        const float base = lv - Rs;
-        tmem_ld_wait();
-        float w[16];
+        for (int b = 4 * hf; b < 4 * hf + 4; ++b) {
+          uint32_t s[16];
+          tmem_ld16(t_s + 16 * (b & 3), s);
+          const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
+          const float base = __shfl_sync(0xffffffffu, lv_lane, 8 + b) - Rs;
+          const float lf = __shfl_sync(0xffffffffu, lf_lane, 8 + b);
+          tmem_ld_wait();
+          float w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = ex2(fmaf(__uint_as_float(s[i]), f, base));
-        if (!all) {
+          for (int i = 0; i < 16; ++i) w[i] = ex2(fmaf(__uint_as_float(s[i]), f, base));
+          if constexpr (!decltype(clean)::value) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * (b >> 1) + key_in_32(16 * (b & 1) + i, b >> 1) >= seen) w[i] = 0.0f;
+            for (int i = 0; i < 16; ++i)
+              if (32 * (b >> 1) + key_in_32(16 * (b & 1) + i, b >> 1) >= seen) w[i] = 0.0f;
+          }
+          float sum[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = (w[i] + w[i + 4]) + (w[i + 8] + w[i + 12]);
+          const float block = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if (decltype(clean)::value || 16 * b < seen) l = fmaf(block, lf, l);
+          if constexpr (!decltype(clean)::value) {
+            if ((zero >> b) & 1u) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+            const float2 back = __half22float2(h);
+            const __half2 m = __floats2half2_rn(w[2 * i] - back.x, w[2 * i + 1] - back.y);
+            s[i] = *reinterpret_cast<const uint32_t*>(&h);
+            s[8 + i] = *reinterpret_cast<const uint32_t*>(&m);
+          }
+          tmem_st16(t_s + 16 * (b & 3), s);
         }
-        float sum[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] = (w[i] + w[i + 4]) + (w[i + 8] + w[i + 12]);
-        if (16 * b < seen)
-          l += ((sum[0] + sum[1]) + (sum[2] + sum[3])) *
-                   ex2(fminf(fmaxf(lv0 - lv, -126.0f), 126.0f)) + poison;
-        if ((zero >> b) & 1u) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
-          const float2 hf2 = __half22float2(h);
-          const __half2 m = __floats2half2_rn(w[2 * i] - hf2.x, w[2 * i + 1] - hf2.y);
-          s[i] = *reinterpret_cast<const uint32_t*>(&h);
-          s[8 + i] = *reinterpret_cast<const uint32_t*>(&m);
-        }
-        tmem_st16(t_s + 16 * (b & 3), s);
-      }
+      };
+      if (is_clean)
+        weights(std::true_type{});
+      else
+        weights(std::false_type{});
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm->p_full[x]);
