@@ -463,7 +463,7 @@ __global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, float* 
   const long long total = q8_locate<32 * kJoinWarps>(sc, item, &front, sh);
   int c0 = 0, c1 = 0;
   if (units) {
-    const long long x0 = front + static_cast<long long>(kvh) * (units + 1) + 1;  // unit 0
+    const long long x0 = front + static_cast<long long>(kvh) * (units + sc.start) + sc.start;  // unit 0
     const int ctas = q8_ctas(sc, total);
     c0 = q8_owner(total, ctas, x0);
     c1 = q8_owner(total, ctas, x0 + units - 1);
@@ -565,7 +565,7 @@ size_t attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int S_max) {
 cudaError_t launch_attention_q8(const float* q, const Q8Cache& c, int n, int H, int seq_len,
                                 const int* lens_dev, float scale, float* out, void* workspace,
                                 cudaStream_t s) {
-  Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, 0, 0, seq_len, lens_dev, 0};
+  Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, 0, 0, 1, seq_len, lens_dev, 0};
   const long long rows = static_cast<long long>(n) * sc.G;
   const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   if (rows > kFewRows)

@@ -45,6 +45,7 @@ constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
 constexpr int kDrain = 4;
+constexpr int kStart = 2;  // places that a pair's query rows and outputs are worth
 constexpr int kBadRow = 0x7FFF;  // exponent of a row of q that is not finite
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
@@ -214,10 +215,10 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         u_first = cur.unit;
         const int w = warp & 7;
 #pragma unroll 1
-        for (int i0 = 0; i0 < 16; i0 += 4) {
-          float4 y[4];
+        for (int i0 = 0; i0 < 16; i0 += 8) {
+          float4 y[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const int qr = cur.tile * kRows + 128 * x + 16 * w + i0 + i;
             const int t = qr / sc.G, g = qr - t * sc.G;
             y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
                   q + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D + 4 * lane));
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const int qrow = 16 * w + i0 + i;
             // the largest magnitude's bits: an infinity or NaN shows as exponent 255
             const uint32_t big = __reduce_max_sync(
@@ -661,54 +662,73 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
   if (warp == 20) tmem_dealloc(tmem, 512);
 }
 
-// k_q8_join for tiles of many rows: a warp per row, few parts each.
-__global__ __launch_bounds__(256) void k_q8_join_rows(Q8Sched sc, float* __restrict__ ws,
-                                                      float* __restrict__ out) {
-  __shared__ long long sh[8 + 1];
-  constexpr int kPer = 32;  // rows of a CTA
-  const int groups = sc.tile_rows / kPer;
-  const int item = blockIdx.x / groups, r0 = blockIdx.x % groups * kPer, kvh = blockIdx.y;
+// k_q8_join for tiles of many rows: a warp per row, few parts each. Small CTAs, of which some find
+// room beside the pass before and work out their place while it runs.
+constexpr int kJoinWarps = 4;
+
+__global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join_rows(Q8Sched sc,
+                                                                  const float* __restrict__ ws_,
+                                                                  float* __restrict__ out) {
+  __shared__ long long sh[kJoinWarps + 1];
+  float* ws = const_cast<float*>(ws_);
+  const int groups = sc.tile_rows / kJoinWarps;
+  const int item = blockIdx.x / groups, kvh = blockIdx.y;
+  const int row = (blockIdx.x - item * groups) * kJoinWarps + (threadIdx.x >> 5);
   const int b = item / sc.tiles, tile = item - b * sc.tiles;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   const int units = q8_units(sc, item);
   long long front;
-  const long long total = q8_locate<256>(sc, item, &front, sh);
+  const long long total = q8_locate<32 * kJoinWarps>(sc, item, &front, sh);
   int c0 = 0, c1 = 0;
   if (units) {
-    const long long x0 = front + static_cast<long long>(kvh) * (units + 1) + 1;  // unit 0
+    const long long x0 = front + static_cast<long long>(kvh) * (units + sc.start) + sc.start;  // unit 0
     const int ctas = q8_ctas(sc, total);
     c0 = q8_owner(total, ctas, x0);
     c1 = q8_owner(total, ctas, x0 + units - 1);
   }
+  const int r = tile * sc.tile_rows + row;
+  const int t = r / sc.G, g = r - t * sc.G;
+  float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D + 4 * lane;
   pdl_wait();
   pdl_launch_dependents();
-  if (units && c0 == c1) return;  // written by its CTA
-  for (int i = warp; i < kPer; i += 8) {
-    const int row = r0 + i, r = tile * sc.tile_rows + row;
-    if (r >= sc.n * sc.G) return;
-    const int t = r / sc.G, g = r - t * sc.G;
-    float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D + 4 * lane;
-    float m = -INFINITY, l = 0.0f;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (units) {
-      for (int c = c0; c <= c1; ++c) {
-        const int slot = 2 * c + (c == c0 ? 1 : 0);
+  if (r >= sc.n * sc.G || (units && c0 == c1)) return;  // one CTA's pair: it is written
+  float m = -INFINITY, l = 0.0f;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int c = c0; units && c <= c1; c += 4) {  // four parts at a time
+    float pm[4], pl[4];
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pm[i] = -INFINITY;
+      pl[i] = 0.0f;
+      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c + i <= c1) {
+        const int slot = 2 * (c + i) + (c + i == c0 ? 1 : 0);
         const float* ml = q8_part_ml(ws, sc.tile_rows, slot);
-        const float pm = ml[row], pl = ml[sc.tile_rows + row];
-        const float4 x = *reinterpret_cast<const float4*>(
+        pm[i] = ml[row];
+        pl[i] = ml[sc.tile_rows + row];
+        x[i] = *reinterpret_cast<const float4*>(
             q8_part_o(ws, sc.tile_rows, slot) + static_cast<size_t>(row) * D + 4 * lane);
-        const float mn = fmaxf(m, pm);
-        // a part without keys, or of NaN scores only, has -inf here
-        const float e0 = m == mn ? 1.0f : ex2(m - mn), e1 = pm == mn ? 1.0f : ex2(pm - mn);
-        l = l * e0 + pl * e1;
-        y = make_float4(y.x * e0 + x.x * e1, y.y * e0 + x.y * e1, y.z * e0 + x.z * e1,
-                        y.w * e0 + x.w * e1);
-        m = mn;
       }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mn = fmaxf(mn, pm[i]);
+    // a part without keys, or of NaN scores only, has -inf for its maximum
+    const float e = m == mn ? 1.0f : ex2(m - mn);
+    l *= e;
+    y = make_float4(y.x * e, y.y * e, y.z * e, y.w * e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = pm[i] == mn ? 1.0f : ex2(pm[i] - mn);
+      l = fmaf(pl[i], f, l);
+      y = make_float4(fmaf(x[i].x, f, y.x), fmaf(x[i].y, f, y.y), fmaf(x[i].z, f, y.z),
+                      fmaf(x[i].w, f, y.w));
+    }
+    m = mn;
   }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
 }  // namespace
@@ -721,7 +741,7 @@ size_t attention_q8_many_workspace_bytes() {
 cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, int H, int seq_len,
                                      const int* lens_dev, float scale_log2, float* out, void* ws,
                                      cudaStream_t s) {
-  Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, kRows, 0, seq_len, lens_dev, 0};
+  Q8Sched sc = {c.B, n, H / c.Hkv, c.Hkv, kRows, 0, kStart, seq_len, lens_dev, 0};
   const long long rows = static_cast<long long>(n) * sc.G;
   sc.tiles = static_cast<int>((rows + kRows - 1) / kRows);
   cudaError_t e = allow_smem<&k_attn_q8_many>(sizeof(ManySmem));
@@ -730,14 +750,14 @@ cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, in
   if (!q8_map(&mk, c.k, c, kUnitKeys) || !q8_map(&mv, c.v, c, kUnitKeys))
     return cudaErrorNotSupported;
   const long long bound = static_cast<long long>(sc.B) * sc.tiles * sc.Hkv *
-                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys + 1);
+                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys + kStart);
   sc.ctas = static_cast<int>(
       std::max<long long>(std::min<long long>(bound, std::min(num_sms_cached(), kManyMaxCtas)), 1));
   e = launch_pdl(&k_attn_q8_many, dim3(sc.ctas), kThreads, sizeof(ManySmem), s, mk, mv, q, c.k_scale,
                  c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, static_cast<float*>(ws));
   if (e != cudaSuccess) return e;
-  return launch_pdl(&k_q8_join_rows, dim3(sc.B * sc.tiles * (kRows / 32), sc.Hkv), 256, 0, s, sc,
-                    static_cast<float*>(ws), out);
+  return launch_pdl(&k_q8_join_rows, dim3(sc.B * sc.tiles * (kRows / kJoinWarps), sc.Hkv),
+                    32 * kJoinWarps, 0, s, sc, static_cast<float*>(ws), out);
 }
 
 }  // namespace obn

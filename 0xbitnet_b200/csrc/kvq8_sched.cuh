@@ -3,8 +3,8 @@
 // The query rows of a sequence and KV head (t * G + g for token t and group head g) are cut
 // into tiles of `tile_rows`; an item is a (sequence, tile), a pair an item with a KV head,
 // and a unit kUnitKeys keys of a pair. Every pair with keys is a start, which costs about as
-// much as a unit (64 sequences of up to 4095: without it the CTAs with 8 short pairs took 41
-// us, those with one 29), and then its units. All places of all pairs in a row, T of them, are
+// much as one unit or two (decode of 64 sequences of up to 4095: without it the CTAs with 8 short
+// pairs took 41 us, those with one 29), and then its units. All places of all pairs in a row, T of them, are
 // dealt out evenly: CTA c of C <= T takes places [c T / C, (c + 1) T / C). So sequences of any
 // mix of lengths and causal tiles of any depth keep every CTA equally busy, and one long
 // sequence is split as finely as many short ones. A pair that lies inside one CTA is written
@@ -26,6 +26,7 @@ constexpr int kQ8MaxCtas = 640;  // bounds C, and with it the workspace
 struct Q8Sched {
   int B, n, G, Hkv;
   int tile_rows, tiles;  // rows per tile, tiles per sequence
+  int start;             // places of a pair's start
   int seq_len;
   const int* lens;
   int ctas;
@@ -45,7 +46,7 @@ OBN_DEVINL int q8_units(const Q8Sched& s, int item) {
   return (max(q8_limit(s, q8_len(s, b), last), 0) + kUnitKeys - 1) / kUnitKeys;
 }
 // Places of a pair of `units` units.
-OBN_DEVINL int q8_places(int units) { return units + (units > 0 ? 1 : 0); }
+OBN_DEVINL int q8_places(const Q8Sched& s, int units) { return units + (units > 0 ? s.start : 0); }
 // CTAs that take part: every one of them has a place.
 OBN_DEVINL int q8_ctas(const Q8Sched& s, long long total) {
   return static_cast<int>(min(static_cast<long long>(s.ctas), total));
@@ -83,7 +84,7 @@ OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* fron
   *i0 = min(tid * per, items);
   *i1 = min(*i0 + per, items);
   long long sum = 0;
-  for (int i = *i0; i < *i1; ++i) sum += q8_places(q8_units(s, i));
+  for (int i = *i0; i < *i1; ++i) sum += q8_places(s, q8_units(s, i));
   sum *= s.Hkv;
   long long incl = sum;
 #pragma unroll
@@ -111,7 +112,7 @@ OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
   int place;
   if (!s.lens && s.tiles == 1) {  // all items alike
     c.units = q8_units(s, 0);
-    const int each = q8_places(c.units);
+    const int each = q8_places(s, c.units);
     const long long total = static_cast<long long>(each) * s.B * s.Hkv;
     const int ctas = q8_ctas(s, total);
     if (static_cast<int>(blockIdx.x) >= ctas) return c;
@@ -137,7 +138,7 @@ OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
     long long* o = sh + THREADS / 32;
     if (x >= at) {  // the thread whose run holds place x walks it
       for (int i = i0; i < i1; ++i) {
-        const int u = q8_units(s, i), each = q8_places(u);
+        const int u = q8_units(s, i), each = q8_places(s, u);
         const long long end = at + static_cast<long long>(each) * s.Hkv;
         if (x < end) {
           // a pair's places times Hkv fit 32 bits: at most 2^23 + 1 units times 65535
@@ -163,12 +164,9 @@ OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
     c.b = c.item / s.tiles;
     c.tile = c.item - c.b * s.tiles;
   }
-  if (place == 0) {  // a start
-    --c.left;
-    c.unit = 0;
-  } else {
-    c.unit = place - 1;
-  }
+  const int skip = max(s.start - place, 0);  // of a start
+  c.left = max(c.left - skip, 0);
+  c.unit = max(place - s.start, 0);
   return c;
 }
 
@@ -177,7 +175,7 @@ OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
 template <int THREADS>
 OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, long long* sh) {
   if (!s.lens && s.tiles == 1) {
-    const long long u = static_cast<long long>(q8_places(q8_units(s, 0))) * s.Hkv;
+    const long long u = static_cast<long long>(q8_places(s, q8_units(s, 0))) * s.Hkv;
     *front = u * item;
     return u * s.B;
   }
@@ -185,7 +183,7 @@ OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, lon
   long long at;
   const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
   if (i0 <= item && item < i1) {
-    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_places(q8_units(s, i))) * s.Hkv;
+    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_places(s, q8_units(s, i))) * s.Hkv;
     sh[THREADS / 32] = at;
   }
   __syncthreads();
@@ -197,7 +195,11 @@ OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, lon
 OBN_DEVINL void q8_next(const Q8Sched& s, Q8Cursor& c) {
   if (--c.left <= 0) return;
   if (++c.unit < c.units) return;
-  if (--c.left == 0) return;  // the next pair's start
+  c.left -= s.start;  // the next pair's
+  if (c.left <= 0) {
+    c.left = 0;
+    return;
+  }
   c.unit = 0;
   if (++c.kvh < s.Hkv) return;
   c.kvh = 0;

@@ -82,17 +82,19 @@ def attention(q, k, v, L, scale):
     G = H // k.shape[1]
     out = np.zeros((n, H, d))
     bound = np.zeros((n, H))
-    for t in range(n):
-        lim = min(L, L - n + t + 1)
-        if lim <= 0:
-            continue
-        for h in range(H):
-            K, V = k[:lim, h // G], v[:lim, h // G]
-            s = K @ q[t, h].astype(np.float64) * scale
-            p = np.exp(s - s.max())
-            out[t, h] = p @ V / p.sum()
-            A = np.max(np.abs(K) @ np.abs(q[t, h].astype(np.float64))) * abs(scale)
-            bound[t, h] = np.abs(V).max() * 2.0 ** -24 * (2 * 48 * A + 64 + lim / 2)
+    lim = np.minimum(L, L - n + np.arange(n) + 1)
+    rows = np.nonzero(lim > 0)[0]
+    if not rows.size:
+        return out, bound
+    hidden = np.arange(L)[None] >= lim[rows][:, None]
+    for h in range(H):
+        K, V, Q = k[:L, h // G], v[:L, h // G], q[rows, h].astype(np.float64)
+        s = np.where(hidden, -np.inf, Q @ K.T * scale)
+        p = np.exp(s - s.max(1, keepdims=True))
+        out[rows, h] = p @ V / p.sum(1, keepdims=True)
+        A = np.where(hidden, 0.0, np.abs(Q) @ np.abs(K).T).max(1) * abs(scale)
+        top = np.maximum.accumulate(np.abs(V).max(1))[lim[rows] - 1]
+        bound[rows, h] = top * 2.0 ** -24 * (2 * 48 * A + 64 + lim[rows] / 2)
     return out, bound
 
 

@@ -188,6 +188,9 @@ def check_attention(torch, rng, B, n, H, Hkv, S, lens=None, sigma=1.0, qs=1.0, p
     (1, 7, 8, 8, 7), (1, 5, 16, 2, 3), (2, 17, 4, 2, 140), (1, 24, 5, 5, 3000),
     (1, 33, 20, 5, 33), (2, 40, 8, 1, 200), (1, 130, 4, 1, 260), (1, 128, 16, 8, 1025),
     (1, 300, 6, 2, 400), (2, 257, 4, 4, 511), (1, 512, 20, 5, 512),
+    # several pairs and many units to a CTA: parts, drained sums, staging reused
+    (40, 300, 4, 1, 700), (150, 64, 2, 2, 640), (1, 512, 20, 5, 2100), (3, 260, 8, 2, 3000),
+    (90, 2, 12, 4, 2000), (300, 1, 8, 8, 400), (60, 4, 16, 4, 1500),
 ])
 def test_attention(B, n, H, Hkv, S):
     torch = need_cuda()
