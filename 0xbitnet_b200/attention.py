@@ -99,11 +99,31 @@ def attention_rope(qkv: torch.Tensor, cache: KVCache, H: int, pos: int,
 Q8_BLOCK = 16  # positions that share a scale
 
 
-def _check_cuda(t, name: str, dtype, device=None) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.is_contiguous()):
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle, without a Stream object
+_current_device = torch._C._cuda_getDevice
+
+
+def _call(name: str, index: int, *args) -> None:
+    """An entry point on device `index` and its current stream (the last argument)."""
+    fn = getattr(lib(), name)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc)
+
+
+def _check(t, name: str, dtype, index: int, numel: int | None = None) -> None:
+    """t is a contiguous tensor of this type (and size) on CUDA device `index`."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype
+            and t.is_contiguous()):
         raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the others are on cuda:{index}")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must hold {numel} elements (got {t.numel()})")
 
 
 class KVCacheQ8:
@@ -125,9 +145,9 @@ class KVCacheQ8:
         """A cache over existing buffers (not copied)."""
         self = cls.__new__(cls)
         for t, name in ((k, "k"), (v, "v")):
-            _check_cuda(t, name, torch.int8, k.device)
+            _check(t, name, torch.int8, k.get_device())
         for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-            _check_cuda(t, name, torch.float32, k.device)
+            _check(t, name, torch.float32, k.get_device())
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k and v must be [B, S_max, Hkv, head_dim], of one shape")
         want = (k.shape[0], -(-k.shape[1] // Q8_BLOCK), k.shape[2])
@@ -139,44 +159,28 @@ class KVCacheQ8:
     def _init(self, k, k_scale, v, v_scale):
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.B, self.S_max, self.Hkv, self.head_dim = k.shape
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.seq_len = 0
 
     def read(self, first: int | torch.Tensor, count: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of rows first .. first + count - 1 of every sequence (an int, or an
         int32 tensor [B] on the device) as f32 k, v [B, count, Hkv, head_dim]; rows outside
         the cache are zero."""
-        k = torch.empty((self.B, count, self.Hkv, self.head_dim), dtype=torch.float32,
-                        device=self.device)
-        v = torch.empty_like(k)
+        shape = (self.B, count, self.Hkv, self.head_dim)
+        k, v = self.k_scale.new_empty(shape), self.k_scale.new_empty(shape)
         host, dev = _host_or_dev(first, self, "first")
-        with _on(self.device):
-            check(lib().obn_kv_read_q8(
-                self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
-                self.v_scale.data_ptr(), self.B, self.Hkv, self.head_dim, self.S_max, host, dev,
-                count, k.data_ptr(), v.data_ptr(), _stream(self.device)))
+        _call("obn_kv_read_q8", self.index, self.k.data_ptr(), self.v.data_ptr(),
+              self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.B, self.Hkv, self.head_dim,
+              self.S_max, host, dev, count, k.data_ptr(), v.data_ptr())
         return k, v
-
-
-def _on(device):
-    """The device as the current one for the launches below."""
-    return torch.cuda.device(device)
 
 
 def _host_or_dev(value, cache: KVCacheQ8, name: str) -> tuple[int, int | None]:
     """(host value, None) of an int, (0, address) of an int32 tensor [B] on the device."""
     if isinstance(value, torch.Tensor):
-        _check_cuda(value, name, torch.int32, cache.device)
-        if value.numel() != cache.B:
-            raise ValueError(f"{name} must hold one value for each of {cache.B} sequences")
+        _check(value, name, torch.int32, cache.index, cache.B)
         return 0, value.data_ptr()
     return int(value), None
-
-
-def _q8_rows(t, name: str, cache: KVCacheQ8, rows: int, cols: int) -> None:
-    _check_cuda(t, name, torch.float32, cache.device)
-    if t.numel() != rows * cols:
-        raise ValueError(f"{name} must be [{rows}, {cols}]")
 
 
 def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
@@ -188,17 +192,15 @@ def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
     the cache are not stored and get a zero q row when pos is a tensor, and are refused when
     it is an int."""
     B, Hkv, d = cache.B, cache.Hkv, cache.head_dim
-    _q8_rows(qkv, "qkv", cache, B * n, (H + 2 * Hkv) * d)
+    _check(qkv, "qkv", torch.float32, cache.index, B * n * (H + 2 * Hkv) * d)
     if q_out is None:
-        q_out = torch.empty((B * n, H * d), dtype=torch.float32, device=cache.device)
+        q_out = qkv.new_empty((B * n, H * d))
     else:
-        _q8_rows(q_out, "q_out", cache, B * n, H * d)
+        _check(q_out, "q_out", torch.float32, cache.index, B * n * H * d)
     host, dev = _host_or_dev(cache.seq_len if pos is None else pos, cache, "pos")
-    with _on(cache.device):
-        check(lib().obn_rope_kv_append_q8(
-            qkv.data_ptr(), B, n, H, Hkv, d, host, dev, theta_base, q_out.data_ptr(),
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), cache.S_max, _stream(cache.device)))
+    _call("obn_rope_kv_append_q8", cache.index, qkv.data_ptr(), B, n, H, Hkv, d, host, dev,
+          theta_base, q_out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+          cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.S_max)
     return q_out
 
 
@@ -219,22 +221,21 @@ def attention_q8(q: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
     tensor [B] on the device, at most max_len, by default the cache's S_max). Query t sees
     keys [0, seq_len - n + t]; one that sees none gives a zero row."""
     B, Hkv, d = cache.B, cache.Hkv, cache.head_dim
-    _q8_rows(q, "q", cache, B * n, H * d)
-    sc = 1.0 / float(np.sqrt(np.float32(d))) if scale is None else scale
+    size = B * n * H * d
+    _check(q, "q", torch.float32, cache.index, size)
     if out is None:
         out = torch.empty_like(q)
     else:
-        _q8_rows(out, "out", cache, B * n, H * d)
+        _check(out, "out", torch.float32, cache.index, size)
     if workspace is None:
         workspace = attention_q8_workspace(cache, H, n)
     else:
-        _check_cuda(workspace, "workspace", torch.uint8, cache.device)
+        _check(workspace, "workspace", torch.uint8, cache.index)
     host, dev = _host_or_dev(seq_len, cache, "seq_len")
     if dev is not None:
         host = cache.S_max if max_len is None else max_len
-    with _on(cache.device):
-        check(lib().obn_attention_q8(
-            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), B, n, H, Hkv, d, cache.S_max, host, dev, sc,
-            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(cache.device)))
+    _call("obn_attention_q8", cache.index, q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+          cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), B, n, H, Hkv, d, cache.S_max, host,
+          dev, d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
+          workspace.numel())
     return out

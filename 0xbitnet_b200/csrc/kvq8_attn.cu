@@ -112,7 +112,10 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   // the lengths may come from the kernel before; the join may read them once all are here
   pdl_wait();
   pdl_launch_dependents();
-  Q8Cursor cur = q8_share<32 * (kWarps + 1)>(sc, sm.sh);
+  int place;
+  long long total;
+  Q8Cursor cur = q8_share<32 * (kWarps + 1)>(sc, blockIdx.x, &place, &total, sm.sh);
+  if (tid == 0) q8_note_split(sc, cur, place, total, ws);
   if (cur.left == 0) return;
   __syncthreads();
   const int H = sc.G * sc.Hkv, rows_seq = sc.n * sc.G;
@@ -442,93 +445,80 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     for (int i = 0; i < min(ST, it); ++i) mbar_wait(&sm.full[i], ((it - 1 - i) / ST) & 1);
 }
 
-// Joins the parts of the pairs that span CTAs, and zeroes the pairs without keys. One CTA per
-// pair and row; first the parts' maxima and totals, a lane a part, then their sums, a warp a
-// part at a time. Where the parts are is worked out while the pass before still runs.
+// Joins the parts of the pairs that span CTAs (q8_note_split), and zeroes the sequences without
+// keys. One CTA per split pair and row (4 rows: all 8 warps to a row; 8 and 16 rows, whose pairs
+// have fewer parts: 2 and 4 rows to a CTA): first the parts' maxima and totals, a lane a part, then
+// their sums, four loads on their way at a time.
 constexpr int kJoinWarps = 8;
 
-__global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, float* __restrict__ ws,
+template <int ROWS>
+__global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, const float* __restrict__ ws_,
                                                              float* __restrict__ out) {
-  __shared__ long long sh[kJoinWarps + 1];
-  __shared__ float s_w[kQ8MaxCtas];  // the parts' weights
+  constexpr int kRowsPer = ROWS / 4, W = kJoinWarps / kRowsPer;  // warps to a row
   __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
   __shared__ float4 s_o[kJoinWarps][32];
-  const int row = blockIdx.x % sc.tile_rows, kvh = blockIdx.y;
-  const int item = blockIdx.x / sc.tile_rows;
-  const int b = item / sc.tiles, tile = item - b * sc.tiles;
-  const int r = tile * sc.tile_rows + row;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int units = q8_units(sc, item);
-  long long front;
-  const long long total = q8_locate<32 * kJoinWarps>(sc, item, &front, sh);
-  int c0 = 0, c1 = 0;
-  if (units) {
-    const long long x0 = front + static_cast<long long>(kvh) * (units + sc.start) + sc.start;  // unit 0
-    const int ctas = q8_ctas(sc, total);
-    c0 = q8_owner(total, ctas, x0);
-    c1 = q8_owner(total, ctas, x0 + units - 1);
-  }
+  float* ws = const_cast<float*>(ws_);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  if (r >= sc.n * sc.G) return;
-  const int t = r / sc.G, g = r - t * sc.G;
-  float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D;
-  if (units == 0) {
-    if (warp == 0) *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    return;
-  }
-  if (c0 == c1) return;  // written by its CTA
-  const int parts = c1 - c0 + 1;
+  if (sc.lens && blockIdx.y == 0) q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
+  const int4 note = *reinterpret_cast<const int4*>(ws + 4 * blockIdx.x);  // item, KV head, last
+  if (note.x < 0) return;
+  const int b = note.x / sc.tiles, tile = note.x - b * sc.tiles;
+  const int c0 = blockIdx.x - 1, parts = note.z - c0 + 1;
   auto slot = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
-  constexpr int kPer = (kQ8MaxCtas + 32 * kJoinWarps - 1) / (32 * kJoinWarps);
-  float pm[kPer], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int i = tid + j * 32 * kJoinWarps;
-    pm[j] = i < parts ? q8_part_ml(ws, sc.tile_rows, slot(i))[row] : -INFINITY;
-    m = fmaxf(m, pm[j]);
-  }
+  const int sub = warp % W;  // of the W warps of a row: parts sub, sub + W, ...
+  const int row = blockIdx.y * kRowsPer + warp / W, r = tile * ROWS + row;
+  float m = -INFINITY, l = 0.0f;
+  for (int i = lane * W + sub; i < parts; i += 32 * W)
+    m = fmaxf(m, q8_part_ml(ws, ROWS, slot(i))[row]);
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, shx(m, d));
-  if (lane == 0) s_m[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, s_m[w]);
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int i = tid + j * 32 * kJoinWarps;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = sub; i0 < parts; i0 += 32 * W) {
+    const int i = i0 + lane * W;
+    float e = 0.0f;
     if (i < parts) {
+      const float* ml = q8_part_ml(ws, ROWS, slot(i));
       // a part of NaN scores only has -inf here and its NaN in the total
-      const float e = pm[j] == m ? 1.0f : ex2(pm[j] - m);
-      s_w[i] = e;
-      l = fmaf(q8_part_ml(ws, sc.tile_rows, slot(i))[sc.tile_rows + row], e, l);
+      e = ml[row] == m ? 1.0f : ex2(ml[row] - m);
+      l = fmaf(ml[ROWS + row], e, l);
+    }
+    const int n = min(32, (parts - i0 + W - 1) / W);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float ek = __shfl_sync(0xffffffffu, e, k);
+      const float4 x = *reinterpret_cast<const float4*>(
+          q8_part_o(ws, ROWS, slot(i0 + k * W)) + row * D + 4 * lane);
+      y = make_float4(fmaf(x.x, ek, y.x), fmaf(x.y, ek, y.y), fmaf(x.z, ek, y.z), fmaf(x.w, ek, y.w));
     }
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) l += shx(l, d);
-  if (lane == 0) s_l[warp] = l;
-  __syncthreads();
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int i = warp; i < parts; i += kJoinWarps) {
-    const float4 x = *reinterpret_cast<const float4*>(
-        q8_part_o(ws, sc.tile_rows, slot(i)) + row * D + 4 * lane);
-    const float e = s_w[i];
-    y = make_float4(fmaf(x.x, e, y.x), fmaf(x.y, e, y.y), fmaf(x.z, e, y.z), fmaf(x.w, e, y.w));
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
   }
   s_o[warp][lane] = y;
   __syncthreads();
-  if (warp) return;
+  if (sub || r >= sc.n * sc.G) return;
+#pragma unroll
+  for (int w = 0; w < W; ++w) m = fmaxf(m, s_m[warp + w]);
   l = 0.0f;
   y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    const float4 x = s_o[w][lane];
-    l += s_l[w];
-    y = make_float4(y.x + x.x, y.y + x.y, y.z + x.z, y.w + x.w);
+  for (int w = 0; w < W; ++w) {
+    // a warp without a part has -inf, no total and no sums
+    const float e = s_m[warp + w] == m ? 1.0f : ex2(s_m[warp + w] - m);
+    const float4 x = s_o[warp + w][lane];
+    l = fmaf(s_l[warp + w], e, l);
+    y = make_float4(fmaf(x.x, e, y.x), fmaf(x.y, e, y.y), fmaf(x.z, e, y.z), fmaf(x.w, e, y.w));
   }
+  const int t = r / sc.G, g = r - t * sc.G;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  *reinterpret_cast<float4*>(
+      out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + note.y * sc.G + g) * D + 4 * lane) =
+      make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
 template <int MT, int KW, int ST, int CTAS>
@@ -547,8 +537,7 @@ cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale
   e = launch_pdl(&k_attn_q8_few<MT, KW, ST, CTAS>, dim3(sc.ctas), 32 * (MT * KW + 1), smem, s, mk, mv,
                  q, c.k_scale, c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, ws);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k_q8_join, dim3(sc.B * sc.tiles * sc.tile_rows, sc.Hkv),
-                    32 * kJoinWarps, 0, s, sc, ws, out);
+  return launch_pdl(&k_q8_join<4 * MT>, dim3(sc.ctas, 4), 32 * kJoinWarps, 0, s, sc, ws, out);
 }
 
 }  // namespace

@@ -169,7 +169,10 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
   const uint32_t tmem = sm->tmem_base;
   pdl_wait();
   pdl_launch_dependents();
-  Q8Cursor cur = q8_share<kThreads>(sc, sm->sh);
+  int place;
+  long long total;
+  Q8Cursor cur = q8_share<kThreads>(sc, blockIdx.x, &place, &total, sm->sh);
+  if (tid == 0) q8_note_split(sc, cur, place, total, ws);
 
   if (cur.left == 0) {
     // nothing for this CTA
@@ -662,73 +665,65 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
   if (warp == 20) tmem_dealloc(tmem, 512);
 }
 
-// k_q8_join for tiles of many rows: a warp per row, few parts each. Small CTAs, of which some find
-// room beside the pass before and work out their place while it runs.
-constexpr int kJoinWarps = 4;
+// k_q8_join for tiles of many rows: a warp per row, few parts each.
+constexpr int kJoinWarps = 8, kJoinRows = 32;
 
 __global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join_rows(Q8Sched sc,
                                                                   const float* __restrict__ ws_,
                                                                   float* __restrict__ out) {
-  __shared__ long long sh[kJoinWarps + 1];
   float* ws = const_cast<float*>(ws_);
-  const int groups = sc.tile_rows / kJoinWarps;
-  const int item = blockIdx.x / groups, kvh = blockIdx.y;
-  const int row = (blockIdx.x - item * groups) * kJoinWarps + (threadIdx.x >> 5);
-  const int b = item / sc.tiles, tile = item - b * sc.tiles;
   const int lane = threadIdx.x & 31;
-  const int units = q8_units(sc, item);
-  long long front;
-  const long long total = q8_locate<32 * kJoinWarps>(sc, item, &front, sh);
-  int c0 = 0, c1 = 0;
-  if (units) {
-    const long long x0 = front + static_cast<long long>(kvh) * (units + sc.start) + sc.start;  // unit 0
-    const int ctas = q8_ctas(sc, total);
-    c0 = q8_owner(total, ctas, x0);
-    c1 = q8_owner(total, ctas, x0 + units - 1);
-  }
-  const int r = tile * sc.tile_rows + row;
-  const int t = r / sc.G, g = r - t * sc.G;
-  float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + kvh * sc.G + g) * D + 4 * lane;
   pdl_wait();
   pdl_launch_dependents();
-  if (r >= sc.n * sc.G || (units && c0 == c1)) return;  // one CTA's pair: it is written
-  float m = -INFINITY, l = 0.0f;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int c = c0; units && c <= c1; c += 4) {  // four parts at a time
-    float pm[4], pl[4];
-    float4 x[4];
+  if (sc.lens && blockIdx.y == 0) q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
+  const int4 note = *reinterpret_cast<const int4*>(ws + 4 * blockIdx.x);  // item, KV head, last
+  if (note.x < 0) return;
+  const int b = note.x / sc.tiles, tile = note.x - b * sc.tiles;
+  const int c0 = blockIdx.x - 1, c1 = note.z;
+#pragma unroll 2
+  for (int i = threadIdx.x >> 5; i < kJoinRows; i += kJoinWarps) {
+    const int row = blockIdx.y * kJoinRows + i, r = tile * sc.tile_rows + row;
+    if (r >= sc.n * sc.G) return;
+    const int t = r / sc.G, g = r - t * sc.G;
+    float* dst = out + ((static_cast<size_t>(b) * sc.n + t) * (sc.G * sc.Hkv) + note.y * sc.G + g) * D + 4 * lane;
+    float m = -INFINITY, l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = c0; c <= c1; c += 4) {  // four parts at a time
+      float pm[4], pl[4];
+      float4 x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pm[i] = -INFINITY;
-      pl[i] = 0.0f;
-      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (c + i <= c1) {
-        const int slot = 2 * (c + i) + (c + i == c0 ? 1 : 0);
-        const float* ml = q8_part_ml(ws, sc.tile_rows, slot);
-        pm[i] = ml[row];
-        pl[i] = ml[sc.tile_rows + row];
-        x[i] = *reinterpret_cast<const float4*>(
-            q8_part_o(ws, sc.tile_rows, slot) + static_cast<size_t>(row) * D + 4 * lane);
+      for (int i = 0; i < 4; ++i) {
+        pm[i] = -INFINITY;
+        pl[i] = 0.0f;
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c + i <= c1) {
+          const int slot = 2 * (c + i) + (c + i == c0 ? 1 : 0);
+          const float* ml = q8_part_ml(ws, sc.tile_rows, slot);
+          pm[i] = ml[row];
+          pl[i] = ml[sc.tile_rows + row];
+          x[i] = *reinterpret_cast<const float4*>(
+              q8_part_o(ws, sc.tile_rows, slot) + static_cast<size_t>(row) * D + 4 * lane);
+        }
       }
-    }
-    float mn = m;
+      float mn = m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mn = fmaxf(mn, pm[i]);
-    // a part without keys, or of NaN scores only, has -inf for its maximum
-    const float e = m == mn ? 1.0f : ex2(m - mn);
-    l *= e;
-    y = make_float4(y.x * e, y.y * e, y.z * e, y.w * e);
+      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, pm[i]);
+      // a part without keys, or of NaN scores only, has -inf for its maximum
+      const float e = m == mn ? 1.0f : ex2(m - mn);
+      l *= e;
+      y = make_float4(y.x * e, y.y * e, y.z * e, y.w * e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = pm[i] == mn ? 1.0f : ex2(pm[i] - mn);
-      l = fmaf(pl[i], f, l);
-      y = make_float4(fmaf(x[i].x, f, y.x), fmaf(x[i].y, f, y.y), fmaf(x[i].z, f, y.z),
-                      fmaf(x[i].w, f, y.w));
+      for (int i = 0; i < 4; ++i) {
+        const float f = pm[i] == mn ? 1.0f : ex2(pm[i] - mn);
+        l = fmaf(pl[i], f, l);
+        y = make_float4(fmaf(x[i].x, f, y.x), fmaf(x[i].y, f, y.y), fmaf(x[i].z, f, y.z),
+                        fmaf(x[i].w, f, y.w));
+      }
+      m = mn;
     }
-    m = mn;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
 }  // namespace
@@ -756,8 +751,7 @@ cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, in
   e = launch_pdl(&k_attn_q8_many, dim3(sc.ctas), kThreads, sizeof(ManySmem), s, mk, mv, q, c.k_scale,
                  c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, static_cast<float*>(ws));
   if (e != cudaSuccess) return e;
-  return launch_pdl(&k_q8_join_rows, dim3(sc.B * sc.tiles * (kRows / kJoinWarps), sc.Hkv),
-                    32 * kJoinWarps, 0, s, sc, static_cast<float*>(ws), out);
+  return launch_pdl(&k_q8_join_rows, dim3(sc.ctas, kRows / kJoinRows), 32 * kJoinWarps, 0, s, sc, static_cast<float*>(ws), out);
 }
 
 }  // namespace obn

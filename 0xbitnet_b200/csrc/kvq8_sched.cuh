@@ -104,50 +104,49 @@ OBN_DEVINL long long q8_scan(const Q8Sched& s, int* i0, int* i1, long long* fron
   return total;
 }
 
-// The first unit of this CTA's share (left 0: it has none). For all threads; sh: THREADS / 32
-// + 8 shared words.
+// The share of CTA `cta` from its first unit on (left 0: it has none). *place: where in its pair
+// the share begins (the start's places, then the units); *total: all places. For all threads;
+// sh: THREADS / 32 + 8 shared words.
 template <int THREADS>
-OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
+OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, int cta, int* place, long long* total, long long* sh) {
   Q8Cursor c = {};
-  int place;
   if (!s.lens && s.tiles == 1) {  // all items alike
     c.units = q8_units(s, 0);
     const int each = q8_places(s, c.units);
-    const long long total = static_cast<long long>(each) * s.B * s.Hkv;
-    const int ctas = q8_ctas(s, total);
-    if (static_cast<int>(blockIdx.x) >= ctas) return c;
-    const long long x = q8_begin(total, ctas, blockIdx.x);
-    c.left = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+    *total = static_cast<long long>(each) * s.B * s.Hkv;
+    const int ctas = q8_ctas(s, *total);
+    if (cta >= ctas) return c;
+    const long long x = q8_begin(*total, ctas, cta);
+    c.left = static_cast<int>(q8_begin(*total, ctas, cta + 1) - x);
     long long pair;
-    if (total <= 0x7FFFFFFFll)
+    if (*total <= 0x7FFFFFFFll)
       pair = static_cast<int>(x) / each;
     else
       pair = x / each;
-    c.item = static_cast<int>(pair) / s.Hkv;
-    c.kvh = static_cast<int>(pair) - c.item * s.Hkv;
-    place = static_cast<int>(x - pair * each);
+    c.item = static_cast<int>(pair / s.Hkv);
+    c.kvh = static_cast<int>(pair - static_cast<long long>(c.item) * s.Hkv);
+    *place = static_cast<int>(x - pair * each);
     q8_enter(s, c);
   } else {
     int i0, i1;
     long long at;
-    const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
-    const int ctas = q8_ctas(s, total);
-    if (static_cast<int>(blockIdx.x) >= ctas) return c;
-    const long long x = q8_begin(total, ctas, blockIdx.x);
-    c.left = static_cast<int>(q8_begin(total, ctas, blockIdx.x + 1) - x);
+    *total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
+    const int ctas = q8_ctas(s, *total);
+    if (cta >= ctas) return c;
+    const long long x = q8_begin(*total, ctas, cta);
+    c.left = static_cast<int>(q8_begin(*total, ctas, cta + 1) - x);
     long long* o = sh + THREADS / 32;
     if (x >= at) {  // the thread whose run holds place x walks it
       for (int i = i0; i < i1; ++i) {
         const int u = q8_units(s, i), each = q8_places(s, u);
         const long long end = at + static_cast<long long>(each) * s.Hkv;
         if (x < end) {
-          // a pair's places times Hkv fit 32 bits: at most 2^23 + 1 units times 65535
-          const unsigned long long in = static_cast<unsigned long long>(x - at);
-          const int kvh = in <= 0x7FFFFFFFull ? static_cast<int>(in) / each
-                                              : static_cast<int>(in / each);
+          const long long in = x - at;
+          const int kvh = in <= 0x7FFFFFFFll ? static_cast<int>(in) / each
+                                             : static_cast<int>(in / each);
           o[0] = i;
           o[1] = kvh;
-          o[2] = static_cast<long long>(in) - static_cast<long long>(kvh) * each;
+          o[2] = in - static_cast<long long>(kvh) * each;
           o[3] = u;
           o[4] = q8_len(s, i / s.tiles);
           break;
@@ -158,37 +157,50 @@ OBN_DEVINL Q8Cursor q8_share(const Q8Sched& s, long long* sh) {
     __syncthreads();
     c.item = static_cast<int>(o[0]);
     c.kvh = static_cast<int>(o[1]);
-    place = static_cast<int>(o[2]);
+    *place = static_cast<int>(o[2]);
     c.units = static_cast<int>(o[3]);
     c.len = static_cast<int>(o[4]);
     c.b = c.item / s.tiles;
     c.tile = c.item - c.b * s.tiles;
   }
-  const int skip = max(s.start - place, 0);  // of a start
+  const int skip = max(s.start - *place, 0);  // of a start
   c.left = max(c.left - skip, 0);
-  c.unit = max(place - s.start, 0);
+  c.unit = max(*place - s.start, 0);
   return c;
 }
 
-// Where the parts of the pairs of item `item` are, for k_q8_join: the total, and in *front the
-// places before the item. For all threads; sh: THREADS / 32 + 1 shared words.
+// The join's work, noted by the CTAs of the pass at the head of the workspace. If the share of
+// CTA j begins inside a pair's units and CTA j - 1 holds the pair's first unit, join CTA j joins
+// that pair: parts of CTAs j - 1 .. last. So each split pair has one join CTA (per row or rows),
+// and there are as many as CTAs, however many pairs there are.
+OBN_DEVINL void q8_note_split(const Q8Sched& s, const Q8Cursor& c, int place, long long total, float* ws) {
+  const int ctas = q8_ctas(s, total), j = blockIdx.x;
+  int4 note = make_int4(-1, 0, 0, 0);  // item (-1: nothing to join), KV head, last CTA
+  if (j > 0 && j < ctas && place > s.start) {
+    const long long x0 = q8_begin(total, ctas, j) - place + s.start;  // unit 0
+    if (q8_owner(total, ctas, x0) == j - 1)
+      note = make_int4(c.item, c.kvh, q8_owner(total, ctas, x0 + c.units - 1), 0);
+  }
+  *reinterpret_cast<int4*>(ws + 4 * j) = note;
+}
+
+// Zeros for the rows of the items without keys, spread over `ctas` CTAs of THREADS threads.
 template <int THREADS>
-OBN_DEVINL long long q8_locate(const Q8Sched& s, int item, long long* front, long long* sh) {
-  if (!s.lens && s.tiles == 1) {
-    const long long u = static_cast<long long>(q8_places(s, q8_units(s, 0))) * s.Hkv;
-    *front = u * item;
-    return u * s.B;
+OBN_DEVINL void q8_zero_empty(const Q8Sched& s, int cta, int ctas, float* out) {
+  const int items = s.B * s.tiles, row4 = s.Hkv * s.G * kQ8HeadDim / 4;
+  for (int i = cta; i < items; i += ctas) {
+    if (q8_units(s, i) > 0) continue;
+    const int b = i / s.tiles, tile = i - b * s.tiles;
+    const int r0 = tile * s.tile_rows, r1 = min(r0 + s.tile_rows, s.n * s.G);
+    // rows r0 .. r1 - 1 of every KV head; a row is 32 pieces of 16 bytes
+    for (long long e = threadIdx.x; e < static_cast<long long>(r1 - r0) * s.Hkv * 32; e += THREADS) {
+      const int piece = static_cast<int>(e % 32), kvh = static_cast<int>(e / 32 % s.Hkv);
+      const int r = r0 + static_cast<int>(e / 32 / s.Hkv), t = r / s.G, g = r - t * s.G;
+      *reinterpret_cast<float4*>(out + (static_cast<size_t>(b) * s.n + t) * row4 * 4 +
+                                 (static_cast<size_t>(kvh) * s.G + g) * kQ8HeadDim + 4 * piece) =
+          make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
   }
-  int i0, i1;
-  long long at;
-  const long long total = q8_scan<THREADS>(s, &i0, &i1, &at, sh);
-  if (i0 <= item && item < i1) {
-    for (int i = i0; i < item; ++i) at += static_cast<long long>(q8_places(s, q8_units(s, i))) * s.Hkv;
-    sh[THREADS / 32] = at;
-  }
-  __syncthreads();
-  *front = sh[THREADS / 32];
-  return total;
 }
 
 // Steps to the share's next unit; left becomes 0 at its end.
@@ -273,16 +285,16 @@ OBN_DEVINL bool q8_wait(volatile int* abort_flag, uint64_t* bar, uint32_t parity
   return false;
 }
 
-// Workspace of a pass of `rows` rows per tile: for each of 2 C slots the sums [rows][128],
-// then the maxima and totals [rows] (all f32).
+// Workspace of a pass of `rows` rows per tile: the notes of the splits; then for each of 2 C
+// slots the sums [rows][128], the maxima and the totals [rows] (all f32).
 OBN_DEVINL float* q8_part_o(float* ws, int rows, int slot) {
-  return ws + static_cast<size_t>(slot) * rows * (kQ8HeadDim + 2);
+  return ws + 4 * kQ8MaxCtas + static_cast<size_t>(slot) * rows * (kQ8HeadDim + 2);
 }
 OBN_DEVINL float* q8_part_ml(float* ws, int rows, int slot) {
   return q8_part_o(ws, rows, slot) + static_cast<size_t>(rows) * kQ8HeadDim;
 }
 constexpr size_t q8_workspace(int rows, int ctas) {
-  return static_cast<size_t>(2) * ctas * rows * (kQ8HeadDim + 2) * sizeof(float);
+  return (4 * kQ8MaxCtas + static_cast<size_t>(2) * ctas * rows * (kQ8HeadDim + 2)) * sizeof(float);
 }
 
 }  // namespace obn

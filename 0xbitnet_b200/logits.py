@@ -11,11 +11,8 @@ import ctypes
 
 import torch
 
-from ._lib import LogitRulesStruct, check, lib
-
-
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+from ._lib import LogitRulesStruct
+from .attention import _call
 
 
 class LogitRules:
@@ -33,10 +30,11 @@ class LogitRules:
     def __init__(self, repetition=None, frequency=None, presence=None, history=None,
                  history_lens=None, bias_ids=None, bias_values=None, bias_lens=None, mask=None):
         self._kept = []     # the tensors whose addresses the struct holds
-        self.device = None
+        self.index = None   # their device
         self.rows = None    # what the per-row tensors agree on
         self.mask_words = 0
         s = self._struct = LogitRulesStruct()
+        self._address = ctypes.addressof(s)
         for name, t in (("repetition", repetition), ("frequency", frequency),
                         ("presence", presence)):
             setattr(s, name, self._vector(t, name, torch.float32))
@@ -55,10 +53,10 @@ class LogitRules:
         if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype
                 and t.is_contiguous()):
             raise TypeError(f"{name} must be a contiguous {dtype} CUDA tensor")
-        if self.device is None:
-            self.device = t.device
-        elif t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, other rules on {self.device}")
+        if self.index is None:
+            self.index = t.get_device()
+        elif t.get_device() != self.index:
+            raise ValueError(f"{name} is on {t.device}, other rules on cuda:{self.index}")
         self._kept.append(t)
 
     def _agree(self, rows, name):
@@ -94,9 +92,9 @@ def logits_process(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | 
             and logits.dtype == torch.float32 and logits.is_contiguous()):
         raise TypeError("logits must be a contiguous torch.float32 CUDA tensor [rows, vocab]")
     rows, vocab = logits.shape
-    device = logits.device
-    if rules.device is not None and rules.device != device:
-        raise ValueError(f"logits are on {device}, the rules on {rules.device}")
+    index = logits.get_device()
+    if rules.index is not None and rules.index != index:
+        raise ValueError(f"logits are on {logits.device}, the rules on cuda:{rules.index}")
     if rules.rows is not None and rules.rows != rows:
         raise ValueError(f"the rules are for {rules.rows} rows, the logits have {rows}")
     if rules.mask_words and rules.mask_words < -(-vocab // 32):
@@ -104,16 +102,14 @@ def logits_process(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | 
                          f"{-(-vocab // 32)}")
     if out is None:
         out = torch.empty_like(logits)
-    elif not (out.shape == logits.shape and out.dtype == torch.float32 and out.is_contiguous()
-              and out.device == device):
+    elif not (out.shape == logits.shape and out.dtype is torch.float32 and out.is_contiguous()
+              and out.is_cuda and out.get_device() == index):
         raise TypeError("out must be like logits")
     if token is None:
-        token = torch.empty(rows, dtype=torch.int32, device=device)
-    elif not (token.numel() == rows and token.dtype == torch.int32 and token.is_contiguous()
-              and token.device == device):
+        token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    elif not (token.numel() == rows and token.dtype is torch.int32 and token.is_contiguous()
+              and token.is_cuda and token.get_device() == index):
         raise TypeError("token must be a contiguous int32 tensor [rows] beside the logits")
-    with torch.cuda.device(device):
-        check(lib().obn_logits_process(logits.data_ptr(), rows, vocab,
-                                       ctypes.addressof(rules._struct), out.data_ptr(),
-                                       token.data_ptr(), _stream(device)))
+    _call("obn_logits_process", index, logits.data_ptr(), rows, vocab, rules._address,
+          out.data_ptr(), token.data_ptr())
     return out, token
