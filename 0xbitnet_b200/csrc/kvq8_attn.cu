@@ -445,9 +445,9 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     for (int i = 0; i < min(ST, it); ++i) mbar_wait(&sm.full[i], ((it - 1 - i) / ST) & 1);
 }
 
-// Joins the parts of the pairs that span CTAs (q8_note_split), and zeroes the sequences without
-// keys. One CTA per split pair and row (4 rows: all 8 warps to a row; 8 and 16 rows, whose pairs
-// have fewer parts: 2 and 4 rows to a CTA): first the parts' maxima and totals, a lane a part, then
+// Joins the parts of the pairs that span CTAs (q8_note_split), and zeroes the items without keys.
+// One CTA per split pair and row (4 rows: all 8 warps to a row; 8 and 16 rows, whose pairs have
+// fewer parts: 2 and 4 rows to a CTA): first the parts' maxima and totals, a lane a part, then
 // their sums, four loads on their way at a time.
 constexpr int kJoinWarps = 8;
 
@@ -461,7 +461,8 @@ __global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join(Q8Sched sc, const f
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  if (sc.lens && blockIdx.y == 0) q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
+  if ((sc.lens || sc.seq_len < sc.n) && blockIdx.y == 0)
+    q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
   const int4 note = *reinterpret_cast<const int4*>(ws + 4 * blockIdx.x);  // item, KV head, last
   if (note.x < 0) return;
   const int b = note.x / sc.tiles, tile = note.x - b * sc.tiles;

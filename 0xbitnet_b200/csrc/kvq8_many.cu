@@ -675,7 +675,8 @@ __global__ __launch_bounds__(32 * kJoinWarps) void k_q8_join_rows(Q8Sched sc,
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  if (sc.lens && blockIdx.y == 0) q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
+  if ((sc.lens || sc.seq_len < sc.n) && blockIdx.y == 0)
+    q8_zero_empty<32 * kJoinWarps>(sc, blockIdx.x, gridDim.x, out);
   const int4 note = *reinterpret_cast<const int4*>(ws + 4 * blockIdx.x);  // item, KV head, last
   if (note.x < 0) return;
   const int b = note.x / sc.tiles, tile = note.x - b * sc.tiles;

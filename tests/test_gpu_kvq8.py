@@ -211,6 +211,22 @@ def test_attention_ragged(n, H, Hkv, lens):
     check_attention(torch, np.random.default_rng(n + H), len(lens), n, H, Hkv, S, lens)
 
 
+@pytest.mark.parametrize("n,H,S", [(1, 4, 0), (8, 4, 3), (40, 4, 0), (300, 4, 7), (520, 2, 100)])
+def test_attention_host_length_shorter_than_the_pass(n, H, S):
+    """Rows before the first position, whole tiles of them too, are zeros."""
+    torch = need_cuda()
+    rng = np.random.default_rng(n + S)
+    cache, k, v = random_cache(torch, rng, 2, 128, 1)
+    q = rng.standard_normal((2 * n, H * D)).astype(np.float32)
+    out = torch.full((2 * n, H * D), float("nan"), device="cuda")
+    att().attention_q8(torch.from_numpy(q).cuda(), cache, H, n, S, out=out)
+    got = out.cpu().numpy().reshape(2, n, H, D)
+    for b in range(2):
+        want, bound = ref.attention(q.reshape(2, n, H, D)[b], k[b], v[b], S, D ** -0.5)
+        assert np.all(got[b][:n - S] == 0)
+        assert np.all(np.abs(got[b] - want).max(-1) <= bound)
+
+
 @pytest.mark.parametrize("n,S", [(1, 900), (3, 900), (64, 300)])
 @pytest.mark.parametrize("qs,sigma", [(0.0, 1.0), (30.0, 4.0), (1e-6, 1.0), (1e5, 2.0 ** -10),
                                       (1.0, 2.0 ** -100)])
