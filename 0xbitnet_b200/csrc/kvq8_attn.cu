@@ -18,9 +18,11 @@
 //    rearrangement (dims may be contracted in any order), V a 4 x 4 byte transpose in
 //    registers (8 byte permutes for 4 keys x 16 dims x 4).
 //  * The s32 sums are carried along the keys and only turned into f32 (and rescaled) when
-//    the reference M has to grow, when a larger value scale comes, or after 2^15 keys (255 *
-//    128 * 2^15 < 2^31). M is set 3 to 4 above the maximum and the scale's reference to 4
-//    times the largest: weights keep 25 bits or more, and few later keys exceed them.
+//    the reference M has to grow, when a weight times its value scale comes above its reference
+//    Vr, or after 2^15 keys (255 * 128 * 2^15 < 2^31). M is set 3 to 4 above the maximum and
+//    Vr to 32 times the largest product: the largest keeps 26 bits or more, and few later keys
+//    exceed them. A value scale alone does not set Vr: a block of large values with small
+//    weights would take bits from the others.
 //  * A producer warp streams 128-key units through a ring of TMA stages, past the ends of
 //    pairs; each consumer warp takes slices of 32 keys of a unit with a softmax state of
 //    its own, and meets the others only at a pair's end, where the states are merged in shared
@@ -327,9 +329,16 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
         float m = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
 #pragma unroll
         for (int d = 4; d <= 16; d <<= 1) m = fmaxf(m, shx(m, d));
-        float vn = sv.x > Vr ? 4.0f * sv.x : Vr;
-        if (second && sv.y > vn) vn = 4.0f * sv.y;
-        flush(m > M ? ceilf(m) + 3.0f : M, vn);
+        const float mn = m > M ? ceilf(m) + 3.0f : M;
+        float top = 0.0f;  // largest weight times value scale
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          if (seen[0][hh]) top = fmaxf(top, ex2(s[0][hh] - mn) * sv.x);
+          if (seen[1][hh]) top = fmaxf(top, ex2(s[1][hh] - mn) * sv.y);
+        }
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, shx(top, d));
+        flush(mn, top > Vr ? 32.0f * top : Vr);
       }
       uint32_t b[2][2];  // weights: [digits 0 1 / 2 3][block]
 #pragma unroll
@@ -384,6 +393,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     const bool whole = pair_ends && u_first == 0;
     if (cur.left > 0) fetch_q();
     flush(M, Vr);
+    if (dead) l = __int_as_float(0x7FC00000);  // no such result passes for one
 #pragma unroll
     for (int d = 4; d <= 16; d <<= 1) l += shx(l, d);
     {

@@ -237,6 +237,31 @@ def test_attention_score_ranges(n, S, qs, sigma):
 
 
 @pytest.mark.parametrize("n", [1, 4, 64])
+def test_attention_large_values_of_small_weight(n):
+    """A block of values 2^24 times the others', with weights below 2^-60, takes no bits from
+    them: the bound counts only the others and the block's own share."""
+    torch = need_cuda()
+    rng = np.random.default_rng(n)
+    S, H, Hkv = 200, 4, 2
+    cache, k, v = random_cache(torch, rng, 1, S, Hkv)
+    q = np.abs(rng.standard_normal((n, H * D))).astype(np.float32) + np.float32(0.5)
+    codes = cache.k.view(1, -1, Hkv, D)
+    codes[:, 64:80] = -127
+    cache.k_scale[:, 4] = 2.0 ** -3
+    k[:, 64:80] = -127 * 2.0 ** -3
+    cache.v_scale[:, 4] = cache.v_scale[:, 4] * 2.0 ** 24
+    v[:, 64:80] *= 2.0 ** 24
+    out = att().attention_q8(torch.from_numpy(q).cuda(), cache, H, n, S)
+    got = out.cpu().numpy().reshape(n, H, D)
+    scale = float(np.float32(1.0) / np.sqrt(np.float32(D)))
+    want, _ = ref.attention(q.reshape(n, H, D), k[0], v[0], S, scale)
+    rest = v[0].copy()
+    rest[64:80] = 0
+    _, bound = ref.attention(q.reshape(n, H, D), k[0], rest, S, scale)
+    assert np.all(np.abs(got - want).max(-1) <= bound)
+
+
+@pytest.mark.parametrize("n", [1, 4, 64])
 def test_attention_zero_and_poisoned_blocks(n):
     """A block of zeros counts with its weight; a NaN scale reaches only the rows that see it."""
     torch = need_cuda()
