@@ -24,6 +24,11 @@ sequence of libobn launches on one stream, so it is captured as a CUDA graph.
 Two or more sequences take the tensor-core LM head (f16 hi/lo split, f32
 accumulation) instead of the shader-order one. Weights are random (seeded)
 with the reference's distributions; no checkpoint is needed to measure speed.
+
+With kv_bits=8 the caches are held in 8 bits (half the bytes, so twice the
+context or sequences), and the sequences may be at positions of their own. pick()
+applies logit rules and leaves each sequence's greedy token as the next step's
+input, so a whole decode iteration is one captured graph without a host read.
 """
 from __future__ import annotations
 
@@ -36,6 +41,7 @@ from . import attention as att
 from ._lib import check, lib
 from .bitlinear import BitLinear, lm_head_f16, lm_head_f16_batched, rmsnorm
 from .diagnose import stage_stats
+from .logits import LogitRules, logits_process
 
 
 # Batches up to this size take the fused RoPE + attention pass (one launch fewer);
@@ -134,11 +140,14 @@ class DecoderLayer:
 
 
 class BitNetDecoder:
-    """B sequences decoding one token per step, KV caches of `ctx` positions."""
+    """B sequences decoding one token per step, KV caches of `ctx` positions in
+    `kv_bits` bits (16: fp16; 8: int8 codes with block scales)."""
 
     def __init__(self, cfg: DecoderConfig, B: int, ctx: int, device=None, seed: int = 0,
-                 keep_source: bool = False):
-        self.cfg, self.B, self.ctx = cfg, B, ctx
+                 keep_source: bool = False, kv_bits: int = 16):
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 16 or 8")
+        self.cfg, self.B, self.ctx, self.kv_bits = cfg, B, ctx, kv_bits
         self.device = device if device is not None else torch.device(
             "cuda", torch.cuda.current_device())
         dev = self.device
@@ -149,7 +158,8 @@ class BitNetDecoder:
             self.embed = (0.02 * torch.randn((cfg.vocab, cfg.hidden), generator=g,
                                              device=dev)).to(torch.float16)
             self.final_norm = _gamma(g, cfg.hidden, dev)
-            self.caches = [att.KVCache(B, ctx, cfg.kv_heads, cfg.head_dim, device=dev)
+            cache = att.KVCache if kv_bits == 16 else att.KVCacheQ8
+            self.caches = [cache(B, ctx, cfg.kv_heads, cfg.head_dim, device=dev)
                            for _ in range(cfg.layers)]
             D, H, d = cfg.hidden, cfg.heads, cfg.head_dim
             f32 = dict(dtype=torch.float32, device=dev)
@@ -161,19 +171,29 @@ class BitNetDecoder:
             self.ffn_out = torch.empty((B, cfg.ffn), **f32)
             self.down_out = torch.empty((B, D), **f32)
             self.ids = torch.zeros((B,), dtype=torch.int32, device=dev)
-            self.attn_ws = torch.empty(max(1, int(lib().obn_attention_workspace_bytes(
-                B, 1, H, d, ctx))), dtype=torch.uint8, device=dev)
+            if kv_bits == 16:
+                self.attn_ws = torch.empty(max(1, int(lib().obn_attention_workspace_bytes(
+                    B, 1, H, d, ctx))), dtype=torch.uint8, device=dev)
+            else:
+                self.attn_ws = att.attention_q8_workspace(self.caches[0], H, 1)
             self.logits = torch.empty((B, cfg.vocab), **f32)
             self.lm_ws = torch.empty(max(1, int(lib().obn_lm_head_workspace_bytes(B, D))),
                                      dtype=torch.uint8, device=dev)
 
     def fill_caches(self, seq_len: int, seed: int = 1) -> None:
-        """Stands in for a prefill: random fp16 keys/values at positions < seq_len."""
+        """Stands in for a prefill: random keys/values at positions < seq_len."""
         g = torch.Generator(device=self.device)
         g.manual_seed(seed)
         for c in self.caches:
-            c.k[:, :seq_len].normal_(generator=g)
-            c.v[:, :seq_len].normal_(generator=g)
+            if self.kv_bits == 16:
+                c.k[:, :seq_len].normal_(generator=g)
+                c.v[:, :seq_len].normal_(generator=g)
+            else:  # about normal values: four standard deviations reach the largest code
+                blocks = -(-seq_len // att.Q8_BLOCK)
+                for codes, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
+                    x = torch.randn(codes[:, :seq_len].shape, generator=g, device=self.device)
+                    codes[:, :seq_len] = (32 * x).round().clamp(-127, 127).to(torch.int8)
+                    scale[:, :blocks] = 1 / 32
             c.seq_len = seq_len
 
     def _embed(self, s) -> None:
@@ -181,16 +201,25 @@ class BitNetDecoder:
         check(lib().obn_embed_f16(_ptr(self.embed), cfg.vocab, cfg.hidden, _ptr(self.ids),
                                   self.B, _ptr(self.x), s))
 
-    def _layer(self, L, c, pos: int) -> None:
+    def _lengths(self, pos):
+        """The sequences' lengths with the step's token, as the attention takes them."""
+        if self.kv_bits == 16 and isinstance(pos, torch.Tensor):
+            raise TypeError("positions per sequence need the 8-bit cache (kv_bits=8)")
+        return pos + 1
+
+    def _layer(self, L, c, pos, lengths) -> None:
         """One transformer block on self.x in place (transformer.rs:51-72)."""
         cfg, B, H = self.cfg, self.B, self.cfg.heads
         L.qkv.forward(self.x, n=B, out=self.qkv_out)
-        if B <= FUSED_ROPE_MAX_BATCH:  # RoPE + KV append + attention in one pass
+        if self.kv_bits == 8:
+            att.rope_kv_append_q8(self.qkv_out, c, H, 1, cfg.rope_theta, q_out=self.q, pos=pos)
+            att.attention_q8(self.q, c, H, 1, lengths, out=self.attn, workspace=self.attn_ws)
+        elif B <= FUSED_ROPE_MAX_BATCH:  # RoPE + KV append + attention in one pass
             att.attention_rope(self.qkv_out, c, H, pos, cfg.rope_theta, out=self.attn,
                                workspace=self.attn_ws)
         else:  # every split CTA would rotate its q heads again: rotate once first
             att.rope_kv_append(self.qkv_out, c, H, 1, cfg.rope_theta, q_out=self.q, pos=pos)
-            att.attention(self.q, c, H, 1, pos + 1, out=self.attn, workspace=self.attn_ws)
+            att.attention(self.q, c, H, 1, lengths, out=self.attn, workspace=self.attn_ws)
         L.o.forward_residual(self.attn, self.x, n=B)  # x += o_proj(attn)
         L.gate_up.forward(self.x, n=B, out=self.ffn_out)
         L.down.forward_residual(self.ffn_out, self.x, n=B)  # x += down(ffn)
@@ -204,15 +233,24 @@ class BitNetDecoder:
         return lm_head_f16_batched(self.embed, self.x, self.final_norm, cfg.eps,
                                    out=self.logits, workspace=self.lm_ws)
 
-    def step(self, pos: int) -> torch.Tensor:
+    def step(self, pos: int | torch.Tensor) -> torch.Tensor:
         """Enqueues one decode step for the tokens in self.ids at position `pos`
-        (every cache holds pos positions before it); returns logits [B, vocab]."""
+        (every cache holds pos positions before it); returns logits [B, vocab].
+        With 8-bit caches pos may be an int32 tensor [B] on the device: a position
+        for each sequence (-1: an idle one, whose cache stays as it is)."""
+        lengths = self._lengths(pos)
         self._embed(_stream(self.device))
         for L, c in zip(self.layers, self.caches):
-            self._layer(L, c, pos)
+            self._layer(L, c, pos, lengths)
         return self._lm_head()
 
-    def diagnose(self, pos: int) -> list[dict]:
+    def pick(self, logits: torch.Tensor, rules: LogitRules) -> torch.Tensor:
+        """Applies the rules to the logits in place and leaves each sequence's
+        greedy token (-1: nothing allowed) in self.ids for the next step."""
+        logits_process(logits, rules, out=logits, token=self.ids)
+        return self.ids
+
+    def diagnose(self, pos: int | torch.Tensor) -> list[dict]:
         """The decode step of `step(pos)`, stage by stage, with the reference's
         diagnostic statistics of each stage (model.ts:449-531): the embedding, the
         hidden state after layers 0 and 1 and after the last layer, the final
@@ -220,12 +258,13 @@ class BitNetDecoder:
         first 100 logits of sequence 0. Synchronises after every stage; the caches
         take the step's k / v as `step` would."""
         cfg = self.cfg
+        lengths = self._lengths(pos)
         host = lambda t: t.detach().float().cpu().numpy()
         out = []
         self._embed(_stream(self.device))
         out.append(stage_stats("embedding", host(self.x)))
         for i, (L, c) in enumerate(zip(self.layers, self.caches)):
-            self._layer(L, c, pos)
+            self._layer(L, c, pos, lengths)
             if i < 2:
                 out.append(stage_stats(f"layer_{i}", host(self.x)))
         out.append(stage_stats("last_layer", host(self.x)))
