@@ -280,8 +280,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
         for (int i = 0; i < 8; ++i) acc[j][i >> 2][i & 3] = 0;
     }
 
-    if (!dead) dead = !mbar_wait(&sm.full[stage], (it / ST) & 1);
-    __syncwarp();
+    if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&sm.full[stage], (it / ST) & 1));
     for (int sub = 0; sub < kSlices; ++sub) {
       const int slice = kw * kSlices + sub;
       const int k0 = cur.unit * kUnitKeys + slice * kSlice;
@@ -338,7 +337,8 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
         }
 #pragma unroll
         for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, shx(top, d));
-        flush(mn, top > Vr ? 32.0f * top : Vr);
+        // only of the rows that need it: no row's bits depend on another's
+        if (mn != M || top > Vr || since >= kFlushSlices) flush(mn, top > Vr ? 32.0f * top : Vr);
       }
       uint32_t b[2][2];  // weights: [digits 0 1 / 2 3][block]
 #pragma unroll
@@ -382,6 +382,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
       }
       ++since;
     }
+    fence_proxy_async_smem();  // read, before a copy writes there again
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.empty[stage]);
 
