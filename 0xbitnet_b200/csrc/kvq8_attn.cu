@@ -555,7 +555,7 @@ cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale
 }  // namespace
 
 // Query rows of a sequence and KV head up to which the few-rows pass runs.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 64;
 
 size_t attention_q8_workspace_bytes(int B, int n, int H, int Hkv, int S_max) {
   (void)B, (void)S_max;

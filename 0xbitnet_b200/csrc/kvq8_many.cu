@@ -46,7 +46,6 @@ constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
 constexpr int kDrain = 4;
 constexpr int kStart = 2;  // places that a pair's query rows and outputs are worth
-constexpr int kBadRow = 0x7FFF;  // exponent of a row of q that is not finite
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
 
@@ -216,59 +215,55 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       q8_next(sc, nxt);
       if (fresh) {  // 16 rows of q a warp, as f16 hi and lo scaled to below 2^14
         u_first = cur.unit;
-        const int w = warp & 7;
+        const int row0 = 16 * (warp & 7), qr0 = cur.tile * kRows + 128 * x + row0;
+        int t = qr0 / sc.G, g = qr0 - t * sc.G;
+        const float* src = q + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D + 4 * lane;
+        int exps = 0;  // of row `lane`
 #pragma unroll 1
         for (int i0 = 0; i0 < 16; i0 += 8) {
           float4 y[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int qr = cur.tile * kRows + 128 * x + 16 * w + i0 + i;
-            const int t = qr / sc.G, g = qr - t * sc.G;
             y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (qr < rows_seq)
-              y[i] = __ldg(reinterpret_cast<const float4*>(
-                  q + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D + 4 * lane));
+            if (qr0 + i0 + i < rows_seq) y[i] = __ldg(reinterpret_cast<const float4*>(src));
+            src += D;
+            if (++g == sc.G) {  // the next token's
+              g = 0;
+              src += (H - sc.G) * D;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int qrow = 16 * w + i0 + i;
-            // the largest magnitude's bits: an infinity or NaN shows as exponent 255
-            const uint32_t big = __reduce_max_sync(
-                0xffffffffu,
-                max(max(__float_as_uint(y[i].x) & 0x7FFFFFFFu, __float_as_uint(y[i].y) & 0x7FFFFFFFu),
-                    max(__float_as_uint(y[i].z) & 0x7FFFFFFFu, __float_as_uint(y[i].w) & 0x7FFFFFFFu)));
-            const bool bad = big >= 0x7F800000u;
-            const int ex = max(static_cast<int>(big >> 23) - 126, -90);  // |q| < 2^ex
+            // An infinity or NaN makes the row's high or low halves NaN, hence its scores.
+            const float big = fmaxf(fmaxf(fabsf(y[i].x), fabsf(y[i].y)), fmaxf(fabsf(y[i].z), fabsf(y[i].w)));
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+            const int ex = max(static_cast<int>(top >> 23) - 126, -90);  // |q| < 2^ex
             const float up = __int_as_float((127 + 14 - ex) << 23);
-            if (lane == 0) sm->q_exp[x][qrow] = static_cast<int16_t>(bad ? kBadRow : ex);
-            uint2 wh = make_uint2(0u, 0u), wl = make_uint2(0u, 0u);
-            if (!bad) {
-              const float e[4] = {y[i].x * up, y[i].y * up, y[i].z * up, y[i].w * up};
-              uint32_t* ph = &wh.x;
-              uint32_t* pl = &wl.x;
+            exps = lane == i0 + i ? ex : exps;
+            const float e[4] = {y[i].x * up, y[i].y * up, y[i].z * up, y[i].w * up};
+            uint32_t wh[2], wl[2];
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
-                const float2 back = __half22float2(h);
-                const __half2 m = __floats2half2_rn(e[2 * j] - back.x, e[2 * j + 1] - back.y);
-                ph[j] = *reinterpret_cast<const uint32_t*>(&h);
-                pl[j] = *reinterpret_cast<const uint32_t*>(&m);
-              }
+            for (int j = 0; j < 2; ++j) {
+              const __half2 h = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
+              const float2 back = __half22float2(h);
+              const __half2 m = __floats2half2_rn(e[2 * j] - back.x, e[2 * j + 1] - back.y);
+              wh[j] = *reinterpret_cast<const uint32_t*>(&h);
+              wl[j] = *reinterpret_cast<const uint32_t*>(&m);
             }
             // 8 bytes of 16-byte chunk (lane / 2) % 8 of the half lane / 16
-            const int at = (lane >> 4) * kHalf + qrow * 128 +
-                           ((((lane >> 1) & 7) ^ (qrow & 7)) << 4) + (lane & 1) * 8;
-            *reinterpret_cast<uint2*>(sm->q[x][0] + at) = wh;
-            *reinterpret_cast<uint2*>(sm->q[x][1] + at) = wl;
+            const int at = (lane >> 4) * kHalf + (row0 + i0 + i) * 128 +
+                           ((((lane >> 1) & 7) ^ (i & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(sm->q[x][0] + at) = make_uint2(wh[0], wh[1]);
+            *reinterpret_cast<uint2*>(sm->q[x][1] + at) = make_uint2(wl[0], wl[1]);
           }
         }
+        if (lane < 16) sm->q_exp[x][row0 + lane] = static_cast<int16_t>(exps);
         fence_proxy_async_smem();
         mbar_arrive(&sm->q_full[x]);
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->q_full[x], pairs & 1));
         if (!ok) break;
         ++pairs;
-        const int qe = sm->q_exp[x][row];
-        sq = (qe == kBadRow ? __int_as_float(0x7FC00000) : __int_as_float((127 + qe - 14) << 23)) * scale_log2;
+        sq = __int_as_float((127 + sm->q_exp[x][row] - 14) << 23) * scale_log2;
         r = cur.tile * kRows + 128 * x + row;
         const bool real = r < rows_seq;
         lim = real ? min(cur.len, q8_limit(sc, cur.len, r)) : 0;
@@ -347,25 +342,32 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
         if (!ok) break;
         tc_fence_after();
-        const float old = copy_R == R ? 1.0f : ex2(copy_R - R);
         const bool add = drain && part_u > kDrain;
-        float4 z[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = add ? __ldcg(copy + i * 128) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (add && copy_R != R) {  // the copy to the reference R
+          const float old = ex2(copy_R - R);
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const float4 z = __ldcg(copy + i * 128);
+            __stcg(copy + i * 128, make_float4(z.x * old, z.y * old, z.z * old, z.w * old));
+          }
+        }
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[16];
           tmem_ld16(t_o + 16 * c, o);
           tmem_ld_wait();
-          if (drain) {  // to the copy, at the reference R; the next piece of it on its way
+          if (drain) {  // added by the L2, which nobody has to wait for
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float4 y = make_float4(fmaf(z[i].x, old, __uint_as_float(o[4 * i])),
-                                           fmaf(z[i].y, old, __uint_as_float(o[4 * i + 1])),
-                                           fmaf(z[i].z, old, __uint_as_float(o[4 * i + 2])),
-                                           fmaf(z[i].w, old, __uint_as_float(o[4 * i + 3])));
-              if (add && c < 3) z[i] = __ldcg(copy + (4 * c + 4 + i) * 128);
-              __stcg(copy + (4 * c + i) * 128, y);
+              float4* at = copy + (4 * c + i) * 128;
+              const float4 y = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                           __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              if (add)
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at),
+                             "f"(y.x), "f"(y.y), "f"(y.z), "f"(y.w)
+                             : "memory");
+              else
+                __stcg(at, y);
             }
           } else {  // to the new reference
 #pragma unroll
@@ -477,15 +479,23 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->staged[x], stagings & 1));
         ++stagings;
         if (!ok) break;
+        const int row0 = 16 * (warp & 7), qr0 = cur.tile * kRows + 128 * x + row0;
+        const int t0 = qr0 / sc.G;
+        int g = qr0 - t0 * sc.G;
+        float* dst = 4 * lane + (whole ? out + ((static_cast<size_t>(cur.b) * sc.n + t0) * H +
+                                                cur.kvh * sc.G + g) * D
+                                       : q8_part_o(ws, kRows, slot) + (128 * x + row0) * D);
+        const int to_next = whole ? (H - sc.G) * D : 0;  // from a token's last row
 #pragma unroll 4
         for (int i = 0; i < 16; ++i) {
-          const int orow = 16 * (warp & 7) + i, qr = cur.tile * kRows + 128 * x + orow;
-          if (qr >= rows_seq) break;
-          const int t = qr / sc.G, g = qr - t * sc.G;
-          float* dst = whole ? out + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G + g) * D
-                             : q8_part_o(ws, kRows, slot) + (128 * x + orow) * D;
-          *reinterpret_cast<float4*>(dst + 4 * lane) =
-              *reinterpret_cast<const float4*>(stage + orow * D + 4 * (lane ^ (orow & 31)));
+          if (qr0 + i >= rows_seq) break;
+          *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(
+              stage + (row0 + i) * D + 4 * (lane ^ ((row0 + i) & 31)));
+          dst += D;
+          if (++g == sc.G) {
+            g = 0;
+            dst += to_next;
+          }
         }
         mbar_arrive(&sm->staged[x]);  // the stage becomes query rows again
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->staged[x], stagings & 1));
