@@ -4,6 +4,7 @@
 // T16 device layout (layout.cuh), workspace partitioning and kernel dispatch.
 // Error handling follows the reference's C ABI: a status return plus a
 // thread-local message (packages/rust/crates/oxbitnet-ffi/src/lib.rs:31-46).
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -907,9 +908,9 @@ int check_q8(const void* k_cache, const void* v_cache, const float* k_scale,
 
 int check_q8_heads(int B, int n, int H, int Hkv) {
   if (n <= 0 || H <= 0) return fail(OBN_ERR_INVALID_ARGUMENT, "need n and H > 0 (got %d, %d)", n, H);
-  if (H % Hkv != 0 || H / Hkv > obn::kQ8MaxGroup)
-    return fail(OBN_ERR_UNSUPPORTED, "H must be 1 to %d times Hkv (got %d / %d)",
-                obn::kQ8MaxGroup, H, Hkv);
+  if (H % Hkv != 0 || H > 65535)
+    return fail(OBN_ERR_UNSUPPORTED, "H must be a multiple of Hkv up to 65535 (got %d / %d)", H,
+                Hkv);
   if (static_cast<long long>(B) * n * H > (1ll << 30))
     return fail(OBN_ERR_UNSUPPORTED, "%d x %d tokens of %d heads are too many", B, n, H);
   return OBN_OK;
@@ -977,6 +978,8 @@ int obn_attention_q8(const float* q, const void* k_cache, const void* v_cache,
   if (seq_len < 0 || seq_len > S_max)
     return fail(OBN_ERR_INVALID_ARGUMENT, "need 0 <= seq_len <= S_max (got %d, %d)", seq_len,
                 S_max);
+  if (!(scale >= 0.0f && scale <= FLT_MAX))
+    return fail(OBN_ERR_INVALID_ARGUMENT, "scale must be finite and not negative");
   const size_t need = obn::attention_q8_workspace_bytes(B, n, H, Hkv, S_max);
   if (workspace_bytes < need)
     return fail(OBN_ERR_INVALID_ARGUMENT, "workspace of %zu bytes is smaller than the %zu needed",

@@ -16,7 +16,6 @@ namespace obn {
 
 constexpr int kQ8HeadDim = 128;  // head_dim the kernels are built for
 constexpr int kQ8Block = 16;     // positions that share a scale
-constexpr int kQ8MaxGroup = 8;   // query heads per KV head
 
 struct Q8Cache {
   int8_t* k;       // [B][S_max][Hkv][128]

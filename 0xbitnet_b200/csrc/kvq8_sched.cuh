@@ -3,14 +3,14 @@
 // The query rows of a sequence and KV head (t * G + g for token t and group head g) are cut
 // into tiles of `tile_rows`; an item is a (sequence, tile), a pair an item with a KV head,
 // and a unit kUnitKeys keys of a pair. Every pair with keys is a start, which costs about as
-// much as one unit or two (decode of 64 sequences of up to 4095: without it the CTAs with 8 short
-// pairs took 41 us, those with one 29), and then its units. All places of all pairs in a row, T of them, are
-// dealt out evenly: CTA c of C <= T takes places [c T / C, (c + 1) T / C). So sequences of any
-// mix of lengths and causal tiles of any depth keep every CTA equally busy, and one long
-// sequence is split as finely as many short ones. A pair that lies inside one CTA is written
-// out by it; the parts of a pair that spans CTAs go to the workspace and are joined by
-// k_q8_join (or k_q8_join_rows). A CTA holds at most two parts: one that continues a pair (slot 2c) and one that
-// begins a pair and does not end it (slot 2c + 1).
+// much as one unit or two (decode of 64 sequences of up to 4095: without it the CTAs with 8
+// short pairs took 41 us, those with one 29), and then its units. All places of all pairs in
+// a row, T of them, are dealt out evenly: CTA c of C <= T takes places [c T / C, (c + 1) T / C).
+// So sequences of any mix of lengths and causal tiles of any depth keep every CTA equally busy,
+// and one long sequence is split as finely as many short ones. A pair that lies inside one CTA
+// is written out by it; the parts of a pair that spans CTAs go to the workspace and are joined by
+// k_q8_join (or k_q8_join_rows). A CTA holds at most two parts: one that continues a pair (slot
+// 2c) and one that begins a pair and does not end it (slot 2c + 1).
 #pragma once
 
 #include "gemm.h"

@@ -311,8 +311,8 @@ OBN_API int obn_attention_decode_rope_at(const float* qkv, void* k_cache, void* 
  * block behind the appended ones keep their codes and lose their meaning: append in order.
  * A token whose position is outside [0, S_max) is stored nowhere and gets a zero q row (left
  * padding and idle sequences: a negative pos_dev[b]); without pos_dev, 0 <= pos and
- * pos + n <= S_max are checked. Needs head_dim == 128, H a multiple of Hkv and
- * H / Hkv <= 8; qkv and q_out 16-byte aligned. */
+ * pos + n <= S_max are checked. Needs head_dim == 128 and H a multiple of Hkv; qkv and
+ * q_out 16-byte aligned. */
 OBN_API int obn_rope_kv_append_q8(const float* qkv, int B, int n, int H, int Hkv, int head_dim,
                                   int pos, const int* pos_dev, float theta_base, float* q_out,
                                   void* k_cache, void* v_cache, float* k_scale, float* v_scale,
@@ -336,9 +336,10 @@ OBN_API size_t obn_attention_q8_workspace_bytes(int B, int n, int H, int Hkv, in
  * (device, [B]) is not NULL: seq_len is then their bound (S_max if nothing better is known;
  * the closer the bound, the better the split). Its query t attends to keys
  * [0, L - n + t]; a query without keys (an empty sequence, left padding) gives a zero row.
- * Sums are exact integers or f32, so results are within f32 rounding of the cache's values.
- * Needs head_dim == 128, H a multiple of Hkv, H / Hkv <= 8 and 0 <= seq_len <= S_max; q and
- * out 16-byte, workspace 256-byte aligned, not used by other work in flight. */
+ * q and the softmax weights enter the products with 22 bits or more, sums are exact integers
+ * or f32: results are near those of f32 arithmetic on the cache's values. Scores have to be
+ * finite in f32. Needs head_dim == 128, H a multiple of Hkv, 0 <= seq_len <= S_max and a finite
+ * scale >= 0; q and out 16-byte, workspace 256-byte aligned, not used by other work in flight. */
 OBN_API int obn_attention_q8(const float* q, const void* k_cache, const void* v_cache,
                              const float* k_scale, const float* v_scale, int B, int n, int H,
                              int Hkv, int head_dim, int S_max, int seq_len,

@@ -88,6 +88,7 @@ def check_append(torch, qkv, cache, H, n, pos, dev_pos):
     (2, 7, 4, 1, [-3, -7], 20, True),        # left padding; nothing at all
     (4, 6, 4, 2, [18, 24, -40, 2147483640], 24, True),  # past the end, idle, far out
     (1, 2, 3, 1, 100001, 100005, False),     # far angles
+    (2, 19, 40, 2, 3, 40, False),            # a large group
 ])
 def test_append(B, n, H, Hkv, pos, S_max, dev_pos):
     torch = need_cuda()
@@ -191,6 +192,9 @@ def check_attention(torch, rng, B, n, H, Hkv, S, lens=None, sigma=1.0, qs=1.0, p
     # several pairs and many units to a CTA: parts, drained sums, staging reused
     (40, 300, 4, 1, 700), (150, 64, 2, 2, 640), (1, 512, 20, 5, 2100), (3, 260, 8, 2, 3000),
     (90, 2, 12, 4, 2000), (300, 1, 8, 8, 400), (60, 4, 16, 4, 1500),
+    # one KV head for many query heads; rows on both sides of the passes' border
+    (2, 1, 20, 1, 300), (1, 1, 71, 1, 500), (1, 3, 24, 2, 700), (3, 16, 4, 1, 90), (1, 13, 5, 1, 333),
+    (2, 4, 48, 3, 150),
 ])
 def test_attention(B, n, H, Hkv, S):
     torch = need_cuda()

@@ -35,7 +35,7 @@ INV, UNS = -1, -2
     ("obn_rope_kv_append_q8", dict(pos=64), INV), ("obn_rope_kv_append_q8", dict(n=65), INV),
     ("obn_rope_kv_append_q8", dict(pos=2147483647), INV),
     ("obn_rope_kv_append_q8", dict(d=64), UNS), ("obn_rope_kv_append_q8", dict(H=5), UNS),
-    ("obn_rope_kv_append_q8", dict(H=18), UNS), ("obn_rope_kv_append_q8", dict(qkv=P + 8), INV),
+    ("obn_rope_kv_append_q8", dict(H=65536), UNS), ("obn_rope_kv_append_q8", dict(qkv=P + 8), INV),
     ("obn_rope_kv_append_q8", dict(q=P + 4), INV), ("obn_rope_kv_append_q8", dict(k=P + 8), INV),
     ("obn_rope_kv_append_q8", dict(base=0.0), INV),
     ("obn_rope_kv_append_q8", dict(base=float("nan")), INV),
@@ -49,7 +49,10 @@ INV, UNS = -1, -2
     ("obn_attention_q8", dict(q=None), INV), ("obn_attention_q8", dict(ws=None), INV),
     ("obn_attention_q8", dict(wb=0), INV), ("obn_attention_q8", dict(ws=P + 128), INV),
     ("obn_attention_q8", dict(L=65), INV), ("obn_attention_q8", dict(L=-1), INV),
-    ("obn_attention_q8", dict(H=3), UNS), ("obn_attention_q8", dict(H=18), UNS),
+    ("obn_attention_q8", dict(H=3), UNS), ("obn_attention_q8", dict(H=65536), UNS),
+    ("obn_attention_q8", dict(scale=-0.5), INV),
+    ("obn_attention_q8", dict(scale=float("nan")), INV),
+    ("obn_attention_q8", dict(scale=float("inf")), INV),
     ("obn_attention_q8", dict(d=96), UNS), ("obn_attention_q8", dict(q=P + 8), INV),
     ("obn_attention_q8", dict(out=P + 4), INV), ("obn_attention_q8", dict(Hkv=0), INV),
     ("obn_attention_q8", dict(n=-1), INV), ("obn_attention_q8", dict(ld=P + 2), INV),
