@@ -83,4 +83,52 @@ cudaError_t allow_smem(size_t bytes) {
   return e;
 }
 
+// How many clusters of `size` CTAs of a kernel (along x, up to 16, which is beyond the portable
+// size) find room on the current device at once. Asked once for each device and size.
+template <auto kKernel>
+int active_clusters(int size, int threads, size_t smem) {
+  static std::atomic<int> known[64][17];  // the answer + 1, 0: not known yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || size < 1 || size > 16) return 0;
+  int n = known[dev][size].load(std::memory_order_relaxed) - 1;
+  if (n >= 0) return n;
+  const void* kernel = reinterpret_cast<const void*>(kKernel);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size, 1);
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess)
+    n = 0;
+  cudaGetLastError();
+  known[dev][size].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
+// launch_pdl with clusters along x.
+template <typename... Args, typename... Given>
+cudaError_t launch_cluster(void (*kernel)(Args...), dim3 grid, int cluster, int threads, size_t smem,
+                           cudaStream_t s, Given&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args>(args)...);
+}
+
 }  // namespace obn

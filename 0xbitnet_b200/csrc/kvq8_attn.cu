@@ -50,6 +50,11 @@ namespace {
 constexpr int D = kQ8HeadDim;
 constexpr int kSlice = 32;                   // keys of a slice: the K of the PV MMA
 constexpr int kTile = kUnitKeys * D;         // bytes of a unit's keys (or values)
+// Units of a CTA up to which a cluster takes a pair. Cluster against dealt-out shares with a join
+// (one token of 20/5 heads, us): 1 sequence of 2048, 4096, 8192 keys 12, 14, 16 against 13, 15, 20,
+// of 16384 (8 units) 20 against 21; 3 sequences of 2048: 14 against 15; 6 of 4096: 18 against 21.
+// 4 tokens of 16/2 heads, 2 sequences of 8192: 22 and 22, of 16384: 31 against 28.
+constexpr int kClusterUnits = 4;
 constexpr int kFlushSlices = 1024;           // 2^15 keys: 255 * 128 * 2^15 < 2^31
 
 // MT tiles of 4 query rows times KW key slices at once: MT * KW consumer warps.
@@ -99,7 +104,31 @@ OBN_DEVINL void cp_async4(uint32_t dst, const float* src, bool in) {  // zeros w
 // one load phase reads differ in bit 2 for K and in bits 1 and 2 for V).
 OBN_DEVINL int key_row(int grp) { return 2 * ((grp >> 1) ^ (2 * (grp & 1))) + (grp & 1); }
 
-template <int MT, int KW, int ST, int CTAS>
+OBN_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+OBN_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// A float (or four) at this CTA's shared address, in the CTA of rank `rank` of the cluster.
+OBN_DEVINL uint32_t in_rank(const void* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+OBN_DEVINL float ld_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+OBN_DEVINL float4 ld_cluster4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
+// With CL a cluster of CTAs takes a pair, an even share of its units each, and joins the parts
+// through its shared memory: one launch, and no shares to work out first.
+template <int MT, int KW, int ST, int CTAS, bool CL>
 __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const float* __restrict__ q, const float* __restrict__ k_scale,
@@ -120,18 +149,29 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   // the lengths may come from the kernel before; the join may read them once all are here
   pdl_wait();
   pdl_launch_dependents();
-  int place;
-  long long total;
-  Q8Cursor cur = q8_share<32 * (kWarps + 1)>(sc, blockIdx.x, &place, &total, sm.sh);
-  if (tid == 0) q8_note_split(sc, cur, place, total, ws);
-  if (cur.left == 0) return;
+  Q8Cursor cur;
+  if constexpr (CL) {
+    cur.item = blockIdx.z;
+    cur.kvh = blockIdx.y;
+    q8_enter(sc, cur);
+    cur.units = q8_units(sc, cur.item);
+    const int rank = blockIdx.x, ranks = gridDim.x;
+    cur.unit = cur.units / ranks * rank + min(rank, cur.units % ranks);
+    cur.left = cur.units / ranks + (rank < cur.units % ranks ? 1 : 0);
+  } else {
+    int place;
+    long long total;
+    cur = q8_share<32 * (kWarps + 1)>(sc, blockIdx.x, &place, &total, sm.sh);
+    if (tid == 0) q8_note_split(sc, cur, place, total, ws);
+    if (cur.left == 0) return;
+  }
   __syncthreads();
   const int H = sc.G * sc.Hkv, rows_seq = sc.n * sc.G;
 
   if (warp == kWarps) {  // producer
     for (int it = 0; cur.left > 0; ++it) {
       const int st = it % ST;
-      if (it >= ST && !__all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (it / ST - 1) & 1))) return;
+      if (it >= ST && !__all_sync(0xffffffffu, mbar_wait(&sm.empty[st], (it / ST - 1) & 1))) break;
       const int k0 = cur.unit * kUnitKeys, left = cur.len - k0;
       const int boxes = min((left + kSlice - 1) / kSlice, kUnitKeys / kSlice);
       if (lane == 0) mbar_arrive_expect_tx(&sm.full[st], boxes * 2 * kSlice * D);
@@ -153,6 +193,12 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
                        smem_u32(&sm.full[st]))
                    : "memory");
       q8_next(sc, cur);
+    }
+    if constexpr (CL) {
+      cluster_arrive();
+      cluster_wait();
+      cluster_arrive();
+      cluster_wait();
     }
     return;
   }
@@ -238,7 +284,16 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
   };
 
-  fetch_q();
+  // The CTA's part of a cluster's pair, in the ring when its units are done: sums [rows][128],
+  // maxima and totals [rows].
+  float* part = reinterpret_cast<float*>(sm.ring[0]);
+  const int item = cur.item, kvh = cur.kvh;
+  if (CL && cur.left == 0) {
+    for (int i = tid; i < kRows * (D + 2); i += 32 * kWarps)
+      part[i] = i >= kRows * D && i < kRows * (D + 1) ? -INFINITY : 0.0f;
+  } else {
+    fetch_q();
+  }
   bool fresh = true;
   int it = 0;
   for (; cur.left > 0; ++it) {
@@ -397,7 +452,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     const bool pair_ends = done.unit + 1 == done.units;
     if (!pair_ends && cur.left > 0) continue;
     // merge the slices, write the pair or its part
-    const bool whole = pair_ends && u_first == 0;
+    const bool whole = !CL && pair_ends && u_first == 0;
     if (cur.left > 0) fetch_q();
     flush(M, Vr);
     if (dead) l = __int_as_float(0x7FC00000);  // no such result passes for one
@@ -416,8 +471,8 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
     }
     consumers();
     const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
-    float* po = q8_part_o(ws, kRows, slot);
-    float* pml = q8_part_ml(ws, kRows, slot);
+    float* po = CL ? part : q8_part_o(ws, kRows, slot);
+    float* pml = CL ? part + kRows * D : q8_part_ml(ws, kRows, slot);
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
       const int row = warp * kRowsPerWarp + i, d4 = 4 * lane;
@@ -460,6 +515,40 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   }
   if (dead)  // a copy may still be on its way into this CTA's shared memory
     for (int i = 0; i < min(ST, it); ++i) mbar_wait(&sm.full[i], ((it - 1 - i) / ST) & 1);
+  if constexpr (CL) {
+    cluster_arrive();
+    cluster_wait();
+    const int ranks = gridDim.x, b = item / sc.tiles, tile = item - b * sc.tiles;
+    for (int row = blockIdx.x + ranks * warp; row < kRows; row += ranks * kWarps) {  // a warp a row
+      const int r = tile * kRows + row;
+      if (r >= rows_seq) break;
+      const bool in = lane < ranks;
+      const float pm = in ? ld_cluster(in_rank(part + kRows * D + row, lane)) : -INFINITY;
+      float l_all = in ? ld_cluster(in_rank(part + kRows * (D + 1) + row, lane)) : 0.0f, m = pm;
+#pragma unroll
+      for (int d = 8; d; d >>= 1) m = fmaxf(m, shx(m, d));
+      // a part without keys, or of NaN scores only, has -inf for its maximum
+      const float e = pm == m ? 1.0f : ex2(pm - m);
+      l_all *= e;
+#pragma unroll
+      for (int d = 8; d; d >>= 1) l_all += shx(l_all, d);
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (int i = 0; i < ranks; ++i) {
+        const float ei = __shfl_sync(0xffffffffu, e, i);
+        const float4 z = ld_cluster4(in_rank(part + row * D + 4 * lane, i));
+        y = make_float4(fmaf(z.x, ei, y.x), fmaf(z.y, ei, y.y), fmaf(z.z, ei, y.z), fmaf(z.w, ei, y.w));
+      }
+      l_all = __shfl_sync(0xffffffffu, l_all, 0);
+      const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key: zeros
+      const int t = r / sc.G, g = r - t * sc.G;
+      *reinterpret_cast<float4*>(
+          out + ((static_cast<size_t>(b) * sc.n + t) * H + kvh * sc.G + g) * D + 4 * lane) =
+          make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    }
+    cluster_arrive();
+    cluster_wait();  // the others have read this CTA's part
+  }
 }
 
 // Joins the parts of the pairs that span CTAs (q8_note_split), and zeroes the items without keys.
@@ -543,17 +632,34 @@ template <int MT, int KW, int ST, int CTAS>
 cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale_log2, float* out,
                        float* ws, cudaStream_t s) {
   constexpr size_t smem = sizeof(FewSmem<MT, KW, ST>);
+  constexpr int threads = 32 * (MT * KW + 1);
   static_assert(CTAS * (smem + 1024) <= 228 * 1024, "shared memory");
-  cudaError_t e = allow_smem<&k_attn_q8_few<MT, KW, ST, CTAS>>(smem);
-  if (e != cudaSuccess) return e;
   CUtensorMap mk, mv;
   if (!q8_map(&mk, c.k, c, kSlice) || !q8_map(&mv, c.v, c, kSlice)) return cudaErrorNotSupported;
-  const long long bound = static_cast<long long>(sc.B) * sc.tiles * sc.Hkv *
-                          ((sc.seq_len + kUnitKeys - 1) / kUnitKeys + 1);
+  const long long pairs = static_cast<long long>(sc.B) * sc.tiles * sc.Hkv;
+  const long long units = (sc.seq_len + kUnitKeys - 1) / kUnitKeys;
   const long long fit = std::min(num_sms_cached() * CTAS, kQ8MaxCtas);
-  sc.ctas = static_cast<int>(std::max<long long>(std::min(bound, fit), 1));
-  e = launch_pdl(&k_attn_q8_few<MT, KW, ST, CTAS>, dim3(sc.ctas), 32 * (MT * KW + 1), smem, s, mk, mv,
-                 q, c.k_scale, c.v_scale, q8_blocks(c.S_max), sc, scale_log2, out, ws);
+  const long long dealt = std::max<long long>(std::min(pairs * (units + 1), fit), 1);
+  if (pairs * ((units + kClusterUnits - 1) / kClusterUnits) <= fit && units <= 16 * kClusterUnits) {
+    constexpr auto* kernel = &k_attn_q8_few<MT, KW, ST, CTAS, true>;
+    cudaError_t e = allow_smem<kernel>(smem);
+    if (e != cudaSuccess) return e;
+    // as many CTAs to a pair as let all pairs run at once
+    for (int size = 16; size * kClusterUnits >= units; size /= 2) {
+      const int ranks = static_cast<int>(std::max<long long>(std::min<long long>(size, units), 1));
+      if (pairs <= active_clusters<kernel>(ranks, threads, smem))
+        return launch_cluster(kernel, dim3(ranks, sc.Hkv, sc.B * sc.tiles), ranks, threads, smem, s,
+                              mk, mv, q, c.k_scale, c.v_scale, q8_blocks(c.S_max), sc, scale_log2,
+                              out, ws);
+      if (size == 1) break;
+    }
+  }
+  constexpr auto* kernel = &k_attn_q8_few<MT, KW, ST, CTAS, false>;
+  cudaError_t e = allow_smem<kernel>(smem);
+  if (e != cudaSuccess) return e;
+  sc.ctas = static_cast<int>(dealt);
+  e = launch_pdl(kernel, dim3(sc.ctas), threads, smem, s, mk, mv, q, c.k_scale, c.v_scale,
+                 q8_blocks(c.S_max), sc, scale_log2, out, ws);
   if (e != cudaSuccess) return e;
   return launch_pdl(&k_q8_join<4 * MT>, dim3(sc.ctas, 4), 32 * kJoinWarps, 0, s, sc, ws, out);
 }

@@ -365,55 +365,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
 cudaError_t launch_logits_process(const float* logits, int rows, int vocab,
                                   const obn_logit_rules& rules, float* out, int32_t* token,
                                   cudaStream_t s) {
-  // Clusters of 16 are beyond the portable size: their place is checked once per device.
   cudaError_t e = allow_smem<&k_logits>(sizeof(LogitSmem));
   if (e != cudaSuccess) return e;
-  static std::atomic<int> largest[64];  // per device, 0: not known yet
-  int dev = 0;
-  e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  int most = dev < 64 ? largest[dev].load(std::memory_order_relaxed) : 8;
-  if (most == 0) {
-    most = 8;
-    if (cudaFuncSetAttribute(k_logits, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
-        cudaSuccess) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(kMaxCluster, 1);
-      cfg.blockDim = kThreads;
-      cfg.dynamicSmemBytes = sizeof(LogitSmem);
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = kMaxCluster;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, k_logits, &cfg) == cudaSuccess && n > 0)
-        most = kMaxCluster;
-    }
-    cudaGetLastError();
-    largest[dev].store(most, std::memory_order_relaxed);
-  }
+  const int most =
+      active_clusters<&k_logits>(kMaxCluster, kThreads, sizeof(LogitSmem)) > 0 ? kMaxCluster : 8;
   // As many CTAs to a row as find room at once, two on an SM.
   const int slices = (vocab + kSliceIds - 1) / kSliceIds;
   int cluster = 1;
   while (cluster < most && cluster < slices && rows * cluster * 2ll <= 2 * num_sms_cached())
     cluster *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster, rows);
-  cfg.blockDim = kThreads;
-  cfg.dynamicSmemBytes = sizeof(LogitSmem);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_logits, logits, vocab, rules, out, token);
+  return launch_cluster(&k_logits, dim3(cluster, rows), cluster, kThreads, sizeof(LogitSmem), s,
+                        logits, vocab, rules, out, token);
 }
 
 }  // namespace obn
