@@ -167,8 +167,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
   // The logit of an id with n occurrences. 1 / rep in f64 serves for the division: quotients
   // of two f32 lie at least 2^-49 (relative) from the middle between two f32, the product is
   // off by 2^-52, so a single occurrence gives the correctly rounded quotient.
+  // A zero or an infinity stays what it is, also where the power leaves f64's range.
   auto penalised = [&](double x, unsigned n) {
-    if (n) x = x * ipow(x > 0.0 ? inv_rep : rep, n) - (freq * n + pres);
+    if (n) {
+      if (x != 0.0 && fabs(x) < INFINITY) x *= ipow(x > 0.0 ? inv_rep : rep, n);
+      x -= freq * n + pres;
+    }
     return x;
   };
 

@@ -103,6 +103,26 @@ def test_single_occurrence_equals_the_sampler():
     assert np.array_equal(out.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("rep", [2.0, 0.5])
+def test_powers_beyond_the_range(rep):
+    """Thousands of occurrences: as dividing or multiplying once for each gives it."""
+    torch = need_cuda()
+    V, n = 40, 3000
+    x = np.array([0.0, -0.0, 3.0, -3.0, np.inf, -np.inf, 1e-40, -1e-40], np.float32)
+    row = np.zeros((1, V), np.float32)
+    row[0, :8] = x
+    r = mod().LogitRules(repetition=torch.full((1,), rep, device="cuda"),
+                         frequency=torch.full((1,), 0.5, device="cuda"),
+                         history=torch.arange(8, dtype=torch.int32, device="cuda").repeat(n))
+    out, _ = mod().logits_process(torch.from_numpy(row).cuda(), r)
+    want = x.astype(np.float64)
+    with np.errstate(over="ignore", under="ignore"):
+        for _ in range(n):
+            want = np.where(want > 0, want / rep, want * rep)
+        want = (want - 0.5 * n).astype(np.float32)
+    assert np.array_equal(out.cpu().numpy()[0, :8], want)
+
+
 def test_special_values_ties_and_empty_rows():
     torch = need_cuda()
     V = 3001
