@@ -27,8 +27,8 @@
 // The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
 // unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 //
-// 2048 rows x 4 of 5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 235 us, 0.46
-// PFLOP/s, 0.92 with the low halves. A unit takes about 9500 cycles, its products 5200: a tile's
+// 2048 tokens of 20/5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 227 us,
+// 0.47 PFLOP/s, 0.94 with the low halves. A unit takes about 9300 cycles, its products 5200: a tile's
 // scores and weights share tensor memory, so its softmax (maximum 900, exchange 600, weights
 // 2700, copies 1100 cycles) and its products (2600) follow one another, and the other tile's
 // products fill only half of the softmax. 512 rows over 2100 keys: 47 us; a pair's query rows and
@@ -51,7 +51,10 @@ namespace {
 constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
-constexpr int kDrain = 4;
+// Units between O's moves to its copy. Error against 64 bits (512 rows over 2100 keys, 2048 over
+// 6144) and time of the latter: 2 units 1.3e-6, 1.4e-6, 236 us; 3: 1.5e-6, 1.6e-6, 227 us; 4: 1.7e-6,
+// 1.9e-6, 219 us; 8: 2.9e-6. An f32 softmax and product of the same values: 1.2e-6, 1.7e-6.
+constexpr int kDrain = 3;
 constexpr int kStart = 2;  // places that a pair's query rows and outputs are worth
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
