@@ -167,7 +167,8 @@ class KVCacheQ8:
         int32 tensor [B] on the device) as f32 k, v [B, count, Hkv, head_dim]; rows outside
         the cache are zero."""
         shape = (self.B, count, self.Hkv, self.head_dim)
-        k, v = self.k_scale.new_empty(shape), self.k_scale.new_empty(shape)
+        k = self.k_scale.new_empty(shape)
+        v = torch.empty_like(k)
         host, dev = _host_or_dev(first, self, "first")
         _call("obn_kv_read_q8", self.index, self.k.data_ptr(), self.v.data_ptr(),
               self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.B, self.Hkv, self.head_dim,
