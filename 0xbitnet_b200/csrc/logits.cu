@@ -18,10 +18,13 @@
 // With the list the f64 work falls on full warps. Histories crowd in a few slices and are
 // sparse in the others: 64 rows of 128256 with 4096 ids took 123 us when the threads that stream
 // the logits rewrote them in passing, 38 us when the threads that count an id rewrote it,
-// 58 us with the history spread over the cluster and remote counters.
+// 58 us with the history spread over the cluster and remote counters, 40 us when the marked ids were
+// gathered and the others streamed through registers past them, without staging; 30 us as it is, 16
+// without any rule. Three smaller slices on their way took 37 us, twice the CTAs 35 us.
 #include "logits.h"
 
 #include <cmath>
+#include <type_traits>
 
 #include "kvq8.h"
 #include "obn_common.cuh"
@@ -100,6 +103,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
   const bool vec_out = (reinterpret_cast<uintptr_t>(y_row) & 15) == (reinterpret_cast<uintptr_t>(x_row) & 15);
   const int end = V + mis;  // positions of the row: [mis, end)
   const int step = cluster * kSliceIds;
+  const int own = 4 * tid - mis;  // the thread's first id in a slice, from the slice's position
+  const int sh = own & 31;        // its bit in a mask word: slices are whole words
   bool dead = false;  // a copy did not come in time: no more of them
 
   // Quads [q_head, q_end) of the slice at p0 lie in the row; one before them and one behind may
@@ -185,21 +190,22 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
     const int cnt = min(kSliceIds, end - p0), nq = (cnt + 3) / 4;
     const bool wait = copied;
     if (p0 + step < end) copied = request(p0 + step, buf ^ 1);
-    // mask words of the thread's quads, used when they have come
+    const int q0 = q_head(p0), q1 = q_end(p0);
+    // mask words of the thread's whole quads, used when they have come: quad k begins at bit sh
+    // of word kThreads / 8 * k behind the first one's
     uint32_t m_lo[kQuads], m_hi[kQuads];
     if (mask) {
+      const uint32_t* words = mask + ((p0 + own) >> 5);
 #pragma unroll
       for (int k = 0; k < kQuads; ++k) {
-        const int q = tid + k * kThreads, v = p0 + 4 * q - mis;
-        const int lo = max(v, 0) >> 5, hi = mis ? min(v + 3, V - 1) >> 5 : lo;
-        m_lo[k] = q < nq ? __ldg(mask + lo) : 0;
-        m_hi[k] = hi != lo && q < nq ? __ldg(mask + hi) : 0;
+        const int q = tid + k * kThreads;
+        m_lo[k] = m_hi[k] = 0;
+        if (q >= q0 && q < q1) {
+          m_lo[k] = __ldg(words + k * (kThreads / 8));
+          if (sh > 28) m_hi[k] = __ldg(words + k * (kThreads / 8) + 1);
+        }
       }
     }
-    auto allowed = [&](int k, int v) {  // bits 0 to 3: of ids v to v + 3
-      if (!mask) return 15u;
-      return v < 0 ? m_lo[k] << -v : __funnelshift_r(m_lo[k], m_hi[k], v & 31);
-    };
     auto in = [&](int at) { return static_cast<unsigned>(at) < static_cast<unsigned>(cnt); };
     // 1. occurrences, distinct ids, biased ids
     if (hist) {
@@ -263,34 +269,42 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
     }
     if (hist || nbias) __syncthreads();
     // 3. out
-    // the quad of the largest logit so far (a NaN is in no maximum and above nothing)
-    auto choose = [&](const float4& y, int v) {
-      const float m = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
-      const bool up = m > best;
-      best = up ? m : best;
-      best_at = up ? v : best_at;
-    };
-    const int q0 = q_head(p0), q1 = q_end(p0);
+    const float* xs = x + 4 * tid;
+    float* ys = y_row + (p0 + own);
+    auto stream = [&](auto masked) {
 #pragma unroll
-    for (int k = 0; k < kQuads; ++k) {
-      const int q = tid + k * kThreads, v = p0 + 4 * q - mis;
-      if (q < q0 || q >= q1) continue;
-      const uint32_t allow = allowed(k, v);
-      float4 y = *reinterpret_cast<const float4*>(x + 4 * q);
-      if (!(allow & 1u)) y.x = -INFINITY;
-      if (!(allow & 2u)) y.y = -INFINITY;
-      if (!(allow & 4u)) y.z = -INFINITY;
-      if (!(allow & 8u)) y.w = -INFINITY;
-      choose(y, v);
-      if (vec_out) {
-        *reinterpret_cast<float4*>(y_row + v) = y;
-      } else {
-        y_row[v] = y.x;
-        y_row[v + 1] = y.y;
-        y_row[v + 2] = y.z;
-        y_row[v + 3] = y.w;
+      for (int k = 0; k < kQuads; ++k) {
+        const int q = tid + k * kThreads;
+        if (q < q0 || q >= q1) continue;
+        float4 y = *reinterpret_cast<const float4*>(xs + 4 * k * kThreads);
+        if constexpr (decltype(masked)::value) {
+          const uint32_t allow = __funnelshift_r(m_lo[k], m_hi[k], sh);  // bits 0 to 3
+          if (!(allow & 1u)) y.x = -INFINITY;
+          if (!(allow & 2u)) y.y = -INFINITY;
+          if (!(allow & 4u)) y.z = -INFINITY;
+          if (!(allow & 8u)) y.w = -INFINITY;
+        }
+        // the quad of the largest logit so far (a NaN is in no maximum and above nothing)
+        const float m = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w));
+        if (m > best) {
+          best = m;
+          best_at = p0 + own + 4 * k * kThreads;
+        }
+        float* dst = ys + 4 * k * kThreads;
+        if (vec_out) {
+          *reinterpret_cast<float4*>(dst) = y;
+        } else {
+          dst[0] = y.x;
+          dst[1] = y.y;
+          dst[2] = y.z;
+          dst[3] = y.w;
+        }
       }
-    }
+    };
+    if (mask)
+      stream(std::true_type{});
+    else
+      stream(std::false_type{});
     if (tid < 8 && (tid < 4 ? q0 > 0 : q1 < nq)) {  // the cut quads, an id a thread
       const int i = 4 * (tid < 4 ? 0 : nq - 1) + (tid & 3), v = p0 + i - mis;
       if (v >= 0 && v < V) {
