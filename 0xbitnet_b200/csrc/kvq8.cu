@@ -252,14 +252,14 @@ __global__ __launch_bounds__(256) void k_read_q8(Q8Cache c, int first, const int
 cudaError_t launch_rope_append_q8(const float* qkv, const Q8Cache& c, int n, int H, int pos,
                                   const int* pos_dev, float theta_base, float* q_out,
                                   cudaStream_t s) {
-  // the frequencies in turns; those of the last theta_base are kept
-  static thread_local RopeTurns turns;
-  static thread_local float turns_base = 0.0f;
-  if (turns_base != theta_base) {
-    for (int i = 0; i < D / 2; ++i)
-      turns.f[i] = std::pow(static_cast<double>(theta_base), -2.0 * i / D) / 6.283185307179586;
-    turns_base = theta_base;
+  // The frequencies in turns, from 16 powers: i = 8 a + b.
+  RopeTurns turns;
+  double coarse[8], fine[8];
+  for (int i = 0; i < 8; ++i) {
+    coarse[i] = std::pow(static_cast<double>(theta_base), -16.0 * i / D) / 6.283185307179586;
+    fine[i] = std::pow(static_cast<double>(theta_base), -2.0 * i / D);
   }
+  for (int i = 0; i < D / 2; ++i) turns.f[i] = coarse[i / 8] * fine[i % 8];
   // blocks that n rows from anywhere inside a block can touch
   const int window = static_cast<int>((static_cast<long long>(n) + 2 * (kQ8Block - 1)) / kQ8Block);
   const long long blocks = static_cast<long long>(window) * c.B;
