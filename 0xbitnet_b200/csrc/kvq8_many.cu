@@ -27,8 +27,8 @@
 // The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
 // unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 //
-// 2048 tokens of 20/5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 227 us,
-// 0.47 PFLOP/s, 0.94 with the low halves. A unit takes about 9300 cycles, its products 5200: a tile's
+// 2048 tokens of 20/5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 222 us,
+// 0.48 PFLOP/s, 0.97 with the low halves. A unit takes about 9100 cycles, its products 5200: a tile's
 // scores and weights share tensor memory, so its softmax (maximum 900, exchange 600, weights
 // 2700, copies 1100 cycles) and its products (2600) follow one another, and the other tile's
 // products fill only half of the softmax. 512 rows over 2100 keys: 47 us; a pair's query rows and
@@ -52,7 +52,7 @@ constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
 // Units between O's moves to its copy. Error against 64 bits (512 rows over 2100 keys, 2048 over
-// 6144) and time of the latter: 2 units 1.3e-6, 1.4e-6, 236 us; 3: 1.5e-6, 1.6e-6, 227 us; 4: 1.7e-6,
+// 6144) and time of the latter: 2 units 1.3e-6, 1.4e-6, 236 us; 3: 1.5e-6, 1.6e-6, 227 us (222 now); 4: 1.7e-6,
 // 1.9e-6, 219 us; 8: 2.9e-6. An f32 softmax and product of the same values: 1.2e-6, 1.7e-6.
 constexpr int kDrain = 3;
 constexpr int kStart = 2;  // places that a pair's query rows and outputs are worth
@@ -137,6 +137,26 @@ OBN_DEVINL void bytes_to_half(uint32_t w, uint32_t* h01, uint32_t* h23) {
   __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), off);
   *h01 = *reinterpret_cast<uint32_t*>(&ha);
   *h23 = *reinterpret_cast<uint32_t*>(&hb);
+}
+
+// q8_wait of the MMA warp, without sleep: it is one warp, and every product waits for it (2048 tokens
+// 227 -> 222 us; softmax warps that spin as well take the slots of those that work: 231 us).
+OBN_DEVINL bool mma_wait(volatile int* abort_flag, uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 24); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 63) == 63 && *abort_flag) return false;
+  }
+  record_error(DEVERR_MBAR_TIMEOUT);
+  *abort_flag = 1;
+  return false;
 }
 
 __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
@@ -613,8 +633,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     int pairs = 0;
     // S of tile x = Q K^T for unit u; `start`: the first of a pair
     auto qk = [&](int x, int u, bool start) {
-      if (x == 0) ok = q8_wait(&sm->abort_flag, &sm->k_full, u & 1);
-      if (ok && start) ok = q8_wait(&sm->abort_flag, &sm->q_full[x], pairs & 1);
+      if (x == 0) ok = mma_wait(&sm->abort_flag, &sm->k_full, u & 1);
+      if (ok && start) ok = mma_wait(&sm->abort_flag, &sm->q_full[x], pairs & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -633,8 +653,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     };
     // O of tile x += P V
     auto pv = [&](int x, int u, bool start) {
-      if (x == 0) ok = q8_wait(&sm->abort_flag, &sm->v_full, u & 1);
-      if (ok) ok = q8_wait(&sm->abort_flag, &sm->p_full[x], u & 1);
+      if (x == 0) ok = mma_wait(&sm->abort_flag, &sm->v_full, u & 1);
+      if (ok) ok = mma_wait(&sm->abort_flag, &sm->p_full[x], u & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
