@@ -15,8 +15,8 @@
 //  * The columns are ordered so that an accumulator quad of a lane is the four digits of one
 //    query row: joining them is lane-local, in the scores and in the sums. Weights go from
 //    there to the B operand of the second product by two shuffles a 16-key block. K needs no
-//    rearrangement (dims may be contracted in any order), V a 4 x 4 byte transpose in
-//    registers (8 byte permutes for 4 keys x 16 dims x 4).
+//    rearrangement (dims may be contracted in any order), V comes transposed from shared memory
+//    (ldmatrix on 16 x 16 bytes; a byte transpose in registers took 36 against 34 us for 8 x 4 tokens).
 //  * The s32 sums are carried along the keys and only turned into f32 (and rescaled) when
 //    the reference M has to grow, when a weight times its value scale comes above its reference
 //    Vr, or after 2^15 keys (255 * 128 * 2^15 < 2^31). M is set 3 to 4 above the maximum and
@@ -31,7 +31,7 @@
 // 64 sequences of up to 4095 keys, 20/5 heads (176 MB): 43 us with the join, 4.0 TB/s, of which
 // about 8 us are starts and the join; the stream itself runs at 5 TB/s. One sequence of 131072
 // (168 MB): 40 us, 4.2 TB/s. 8 sequences of up to 5000 with 32 rows (24 MB): 33 us, where the
-// warps issue: 16 rows cost 1.6 times what 8 do. 12 warps an SM (3 CTAs whose first warp
+// products bound the warps: 16 rows cost 1.6 times what 8 do, half of V's products less 8 us less. 12 warps an SM (3 CTAs whose first warp
 // requests the units between its own) took 51, 42 and 37 us.
 #include "kvq8.h"
 
@@ -85,6 +85,15 @@ OBN_DEVINL void mma_su8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Two 16 x 16 tiles of bytes, transposed: lane i < 16 gives the address of row i of the first, lane
+// 16 + i of the second. a[0], a[1]: columns grp and grp + 8 of rows 4 qd .. 4 qd + 3 of the first,
+// a[2], a[3] of the second, an s8 MMA's A operand.
+OBN_DEVINL void ld_transposed(uint32_t (&a)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+               : "r"(addr)
+               : "memory");
+}
 // An overflowed score stays the largest or smallest number, a NaN stays one.
 OBN_DEVINL float clamp_score(float x) {
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(FLT_MAX));
@@ -100,8 +109,8 @@ OBN_DEVINL void cp_async4(uint32_t dst, const float* src, bool in) {  // zeros w
 
 // Row (of a block of 16) behind row `grp` (0 .. 7) of an MMA's A operand; row grp + 8 is 8
 // further on. The order is free as long as K, the weights and V agree; with this one the
-// 16-byte fragment loads run over the 128-byte swizzle without bank conflicts (the rows that
-// one load phase reads differ in bit 2 for K and in bits 1 and 2 for V).
+// 16-byte fragment loads of K run over the 128-byte swizzle without bank conflicts (the rows that
+// one load phase reads differ in bit 2); V's rows are those of the weights' order.
 OBN_DEVINL int key_row(int grp) { return 2 * ((grp >> 1) ^ (2 * (grp & 1))) + (grp & 1); }
 
 OBN_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -208,12 +217,8 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   // this lane's fragments: K row and the two chunks of it, V rows of its key quad
   const int kr = key_row(grp);
   const uint32_t k_off = kr * D + ((qd ^ (kr & 7)) << 4);  // chunk qd + 4: ^ 64
-  uint32_t v_off[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int vr = key_row(2 * qd + e);
-    v_off[e] = kTile + vr * D + ((grp ^ (vr & 7)) << 4);
-  }
+  const int vr = 16 * (lane >> 4) + 8 * (lane & 1) + key_row((lane & 15) >> 1);
+  const uint32_t v_off = kTile + vr * D;
   // selectors of the weights' way to the B operand
   const bool odd = grp & 1;
   const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
@@ -221,8 +226,8 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
   const int src_b = (2 * qd + (odd ? 0 : 1)) * 4 + (grp >> 1);
 
   bool dead = false;  // a copy did not come in time: no more waits
-  int acc[8][2][4];   // [dim pair tile][digits 0 1 / 2 3][dim 0: 2 digits, dim 1: 2 digits]
-  float o[16];        // dims 16 grp .. + 15 of query row qd of the tile
+  int acc[8][2][4];   // [16 dims][digits 0 1 / 2 3][dim grp: 2 digits, dim grp + 8: 2 digits]
+  float o[16];        // dims grp, grp + 8, .. of query row qd of the tile
   float M = -INFINITY, l = 0.0f, Vr = 0.0f, inv_vr = 0.0f, sq = 0.0f;
   int lim = 0, since = 0, most = 0, u_first = 0;
   uint32_t bq[4][2][2];  // q: [k step][digits 0 1 / 2 3][dims 16 qd + 4 k / 64 + 16 qd + 4 k]
@@ -422,24 +427,12 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
         b[0][kb] = __byte_perm(za, zb, sel_lo);
         b[1][kb] = __byte_perm(za, zb, sel_hi);
       }
-      uint4 v[2][4];  // [block][key of the quad]
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int j = 0; j < 8; ++j) {  // 16 dims x 32 keys
+        uint32_t a[4];
+        ld_transposed(a, smem_u32(st) + v_off + ((j ^ (vr & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[kb][i] = *reinterpret_cast<const uint4*>(st + (kb * 16 + (i & 1) * 8) * D + v_off[i >> 1]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        auto word = [&](const uint4& x) { return w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w; };
-        uint32_t t0[4], t1[4];
-        transpose4(word(v[0][0]), word(v[0][1]), word(v[0][2]), word(v[0][3]), t0);
-        transpose4(word(v[1][0]), word(v[1][1]), word(v[1][2]), word(v[1][3]), t1);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t a[4] = {t0[2 * e], t0[2 * e + 1], t1[2 * e], t1[2 * e + 1]};
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) mma_su8(acc[2 * w + e][nt], a, b[nt][0], b[nt][1]);
-        }
+        for (int nt = 0; nt < 2; ++nt) mma_su8(acc[j][nt], a, b[nt][0], b[nt][1]);
       }
       ++since;
     }
@@ -465,9 +458,7 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
         sm.l[kw][row] = l;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(&sm.o[kw][row][16 * grp + 4 * i]) =
-            make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      for (int i = 0; i < 16; ++i) sm.o[kw][row][8 * i + grp] = o[i];
     }
     consumers();
     const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
@@ -657,7 +648,8 @@ cudaError_t launch_few(const float* q, const Q8Cache& c, Q8Sched sc, float scale
   constexpr auto* kernel = &k_attn_q8_few<MT, KW, ST, CTAS, false>;
   cudaError_t e = allow_smem<kernel>(smem);
   if (e != cudaSuccess) return e;
-  sc.ctas = static_cast<int>(dealt);
+  // The heads of a long sequence in step, on the same rows of memory (131072 keys: 53 -> 51 us).
+  sc.ctas = static_cast<int>(dealt >= sc.Hkv ? dealt / sc.Hkv * sc.Hkv : dealt);
   e = launch_pdl(kernel, dim3(sc.ctas), threads, smem, s, mk, mv, q, c.k_scale, c.v_scale,
                  q8_blocks(c.S_max), sc, scale_log2, out, ws);
   if (e != cudaSuccess) return e;
