@@ -31,7 +31,7 @@
 // 64 sequences of up to 4095 keys, 20/5 heads (176 MB): 43 us with the join, 4.0 TB/s, of which
 // about 8 us are starts and the join; the stream itself runs at 5 TB/s. One sequence of 131072
 // (168 MB): 40 us, 4.2 TB/s. 8 sequences of up to 5000 with 32 rows (24 MB): 33 us, where the
-// products bound the warps: 16 rows cost 1.6 times what 8 do, half of V's products less 8 us less. 12 warps an SM (3 CTAs whose first warp
+// products bound the warps: 16 rows cost 1.6 times what 8 do, and half of V's products cost 8 us. 12 warps an SM (3 CTAs whose first warp
 // requests the units between its own) took 51, 42 and 37 us.
 #include "kvq8.h"
 
