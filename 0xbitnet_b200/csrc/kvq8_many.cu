@@ -23,7 +23,12 @@
 // is w = 2^(s f + lv - R), so its f16 pair is as exact as the contribution it makes is large,
 // whatever the scales of other blocks, and O adds w times codes. R moves only when a row's
 // maximum of s f + lv exceeds it by 15 (w <= 2^15 fits f16); then O is rescaled in
-// tensor memory. The total is the sum of w 2^(lv0 - lv), exact factors, lv0 fixed for a part.
+// tensor memory. The total is the sum of w 2^(lv0 - lv), exact factors, lv0 fixed for a part, while
+// every value scale of the part lies within 2^32 of 2^lv0: its reference is T = R - lv0 then, and no
+// weight that counts is flushed (R <= max s f + lv0 + 26, so a score 60 below the largest still has
+// w >= 2^-118). From the first unit with a scale farther off, or with a block of zeros (whose keys
+// have weight but no product), the rest of the part is `far`: the total has exponentials and a
+// reference T of its own, moved like R but by the scores alone, and R goes by the other blocks.
 // The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
 // unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 //
@@ -55,6 +60,8 @@ constexpr int kThreads = 672;
 // 6144) and time of the latter: 2 units 1.3e-6, 1.4e-6, 236 us; 3: 1.5e-6, 1.6e-6, 227 us (222 now); 4: 1.7e-6,
 // 1.9e-6, 219 us; 8: 2.9e-6. An f32 softmax and product of the same values: 1.2e-6, 1.7e-6.
 constexpr int kDrain = 3;
+constexpr float kNear = 32.0f;  // how far from lv0 a value scale's exponent may be
+constexpr float kNoExp = -1000.0f;  // the exponent of a scale of zero
 constexpr int kStart = 2;  // places that a pair's query rows and outputs are worth
 constexpr int kManyMaxCtas = 160;
 constexpr int kHalf = 128 * 128;  // bytes of 128 rows x 64 f16, the swizzle's width
@@ -159,6 +166,34 @@ OBN_DEVINL bool mma_wait(volatile int* abort_flag, uint64_t* bar, uint32_t parit
   return false;
 }
 
+// The total of a far part, over the 64 scores of a thread's half of a unit: l counts in 2^T, and T
+// moves like R. Each half has a T of its own.
+OBN_DEVINL void add_far(uint32_t t_s, int hf, float sq, float scl, int seen, float* T, float* l) {
+#pragma unroll 1
+  for (int b = 4 * hf; b < 4 * hf + 4; ++b) {
+    const float f = sq * __shfl_sync(0xffffffffu, scl, b);
+    const float sv = __shfl_sync(0xffffffffu, scl, 8 + b);
+    uint32_t s[16];
+    tmem_ld16(t_s + 16 * (b & 3), s);
+    tmem_ld_wait();
+    float top = -INFINITY, block = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (32 * (b >> 1) + key_in_32(16 * (b & 1) + i, b >> 1) < seen)
+        top = fmaxf(top, __uint_as_float(s[i]) * f);
+    if (top > *T + 15.0f) {
+      const float to = ceilf(top) - 7.0f;
+      *l *= ex2(*T - to);
+      *T = to;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (32 * (b >> 1) + key_in_32(16 * (b & 1) + i, b >> 1) < seen)
+        block += ex2(fmaf(__uint_as_float(s[i]), f, -*T));
+    if (16 * b < seen) *l += block + (sv - sv);  // a poisoned block makes it NaN
+  }
+}
+
 __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
     const float* __restrict__ q, const float* __restrict__ k_scale,
@@ -215,11 +250,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
     // the copy of O: [4 dims] of this half, row by row
     float4* copy = reinterpret_cast<float4*>(ws + q8_workspace(kRows, kManyMaxCtas) / sizeof(float)) +
                    ((static_cast<size_t>(blockIdx.x) * 2 + x) * 2 + hf) * (16 * 128) + row;
-    float R = -INFINITY, l = 0.0f, lv0 = 0.0f, sq = 0.0f, scl = 0.0f, copy_R = 0.0f;
+    float R = -INFINITY, l = 0.0f, lv0 = 0.0f /* T in a far part */, sq = 0.0f, scl = 0.0f, copy_R = 0.0f;
     int part_u = 0;  // units of the part so far
     uint32_t swaps = 0, stagings = 0;
     int lim = 0, u_first = 0, r = 0, pairs = 0;
-    bool fresh = true, ok = true;
+    bool fresh = true, ok = true, far = false;
     // lanes 0-7: the unit's key scales, 8-15: its value scales
     auto load_scale = [&](const Q8Cursor& c) {
       const int blk = c.unit * (kUnitKeys / kQ8Block) + (lane & 7);
@@ -228,14 +263,15 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
                          (static_cast<size_t>(c.b) * nblk + blk) * sc.Hkv + c.kvh)
                  : 0.0f;
     };
-    // this half's value to the other one's thread, and back; false after an abort
+    // this half's value to the other one's thread, and back; false after an abort. The halves change
+    // slots each time: a slot is next written by the thread that read it.
     auto exchange = [&](float mine, float* other) {
-      sm->swapped[x][hf][row] = mine;
+      sm->swapped[x][hf ^ (swaps & 1)][row] = mine;
       mbar_arrive(&sm->swap[x][warp & 3]);
       const bool came =
           __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->swap[x][warp & 3], swaps & 1));
+      *other = sm->swapped[x][hf ^ 1 ^ (swaps & 1)][row];
       ++swaps;
-      *other = sm->swapped[x][hf ^ 1][row];
       return came;
     };
     scl = load_scale(cur);
@@ -300,19 +336,23 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         R = -INFINITY;
         l = 0.0f;
         part_u = 0;
+        far = false;
         // the reference of the value scales: the unit's largest exponent
         float top = lane >= 8 && lane < 16 && scl > 0.0f ? scl : 0.0f;
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         lv0 = top > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127) : 0.0f;
       }
-      // exponents of the value scales (of zero and poisoned blocks: any, the weights of a zero
-      // one are left out of P and count in the total)
-      const bool plain = scl > 0.0f;
+      // exponents of the value scales (a poisoned block's: any, it makes the total NaN)
       const float lv_lane =
-          plain ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127) : lv0;
+          scl > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127)
+                     : scl == 0.0f ? kNoExp : lv0;
+      if (!far && __any_sync(0xffffffffu, lane >= 8 && lane < 16 && k0 + kQ8Block * (lane & 7) < cur.len &&
+                                              fabsf(lv_lane - lv0) > kNear)) {
+        far = true;
+        lv0 = R == -INFINITY ? R : R - lv0;  // what l counts in
+      }
       // a block's part of the total counts times this: 2^(lv0 - lv), NaN for a poisoned one
-      const float lf_lane = ex2(fminf(fmaxf(lv0 - lv_lane, -126.0f), 126.0f)) + (scl - scl);
-      const uint32_t zero = (__ballot_sync(0xffffffffu, scl == 0.0f) >> 8) & 255u;
+      const float lf_lane = ex2(lv0 - lv_lane) + (scl - scl);
       const float scl_now = scl;
       if (nxt.left > 0) scl = load_scale(nxt);
 
@@ -321,11 +361,13 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->s_full[x], u & 1));
       if (!ok) break;
       tc_fence_after();
+      if (__builtin_expect(far, false)) add_far(t_s, hf, sq, scl_now, seen, &lv0, &l);
       // 1. the largest s f + lv of the row. The loops over 16-key blocks stay loops: unrolled, the
       // softmax warps, the converters and the MMA warp evict each other's instructions (both
       // passes unrolled: 8600 cycles a unit; in halves: 5600).
-      // Units where nothing is masked and no block is zero have code of their own: compiled as
-      // one, the masks cost every element two selects and two compares.
+      // Units where nothing is masked or far have code of their own: compiled as one, the masks
+      // cost every element two selects and two compares. (With a third version for far parts, in
+      // place of add_far, the others ran slower too: 2048 rows 251 -> 276 us, as it is 257.)
       float xr = -INFINITY;
       auto largest = [&](auto clean) {
 #pragma unroll 1
@@ -355,7 +397,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
           xr = fmaxf(xr, m1 == -INFINITY ? -INFINITY : fmaf(m1, f1, lv_1));
         }
       };
-      const bool is_clean = all && zero == 0;
+      const bool is_clean = all && !far;
       if (is_clean)
         largest(std::true_type{});
       else
@@ -367,7 +409,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       const float Rn = grow ? ceilf(xr) - 7.0f : R;
       const float corr = grow ? ex2(R - Rn) : 1.0f;
       const bool drain = part_u > 0 && part_u % kDrain == 0;
-      l *= corr;
+      l *= far ? 1.0f : corr;
       if (part_u > 0 && (drain || __any_sync(0xffffffffu, grow))) {
         ok = __all_sync(0xffffffffu, q8_wait(&sm->abort_flag, &sm->o_full[x], (u - 1) & 1));
         if (!ok) break;
@@ -421,7 +463,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
           uint32_t s[16];
           tmem_ld16(t_s + 16 * (b & 3), s);
           const float f = sq * __shfl_sync(0xffffffffu, scl_now, b);
-          const float base = __shfl_sync(0xffffffffu, lv_lane, 8 + b) - Rs;
+          const float lv = __shfl_sync(0xffffffffu, lv_lane, 8 + b), base = lv - Rs;
           const float lf = __shfl_sync(0xffffffffu, lf_lane, 8 + b);
           tmem_ld_wait();
           float w[16];
@@ -436,9 +478,9 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] = (w[i] + w[i + 4]) + (w[i + 8] + w[i + 12]);
           const float block = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          if (decltype(clean)::value || 16 * b < seen) l = fmaf(block, lf, l);
+          if (decltype(clean)::value || (!far && 16 * b < seen)) l = fmaf(block, lf, l);
           if constexpr (!decltype(clean)::value) {
-            if ((zero >> b) & 1u) {
+            if (lv == kNoExp) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) w[i] = 0.0f;
             }
@@ -468,14 +510,27 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
         if (!ok) break;
         tc_fence_after();
         float lo;
+        if (far) {
+          if (!exchange(lv0, &lo)) break;
+          const float T = fmaxf(lv0, lo);
+          if (lv0 != T) l *= ex2(lv0 - T);
+          lv0 = T;
+        }
         if (!exchange(l, &lo)) break;
         l = hf ? lo + l : l + lo;
         const bool whole = pair_ends && u_first == 0;
         const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
-        const float unit = ex2(lv0) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
+        // O counts in 2^R and the total in 2^T. A total goes on as 1 <= l < 2 times 2^e, and the sums
+        // of a part as that much less, so that neither leaves f32's range before the result does.
+        const float T = far ? lv0 : R == -INFINITY ? R : R - lv0;
+        const int e = l > 0.0f && l <= FLT_MAX ? static_cast<int>(__float_as_uint(l) >> 23) - 127 : 0;
+        l *= ex2(static_cast<float>(-e));
+        const float up = (R == -INFINITY ? 0.0f : R - T) - static_cast<float>(e);
+        const float near_up = fminf(fmaxf(up, -100.0f), 100.0f), rest_up = ex2(up - near_up);
+        const float unit = ex2(near_up) * (whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f);
         if (!whole && hf == 0) {
           float* ml = q8_part_ml(ws, kRows, slot);
-          ml[128 * x + row] = R == -INFINITY ? -INFINITY : R - lv0;
+          ml[128 * x + row] = T + static_cast<float>(e);
           ml[kRows + 128 * x + row] = l;
         }
         const bool copied = part_u > kDrain;
@@ -502,7 +557,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
                                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
             const int piece = 16 * hf + 4 * c + i;
             *reinterpret_cast<float4*>(stage + row * D + 4 * (piece ^ (row & 31))) =
-                make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
+                make_float4(y.x * unit * rest_up, y.y * unit * rest_up, y.z * unit * rest_up,
+                            y.w * unit * rest_up);
           }
         }
         mbar_arrive(&sm->staged[x]);

@@ -98,6 +98,41 @@ def attention(q, k, v, L, scale):
     return out, bound
 
 
+def attention_by_products(q, k, v, v_scale, L, scale):
+    """attention() with a bound on each output element [n, H, d] that goes by what adds up to it,
+    for caches whose value scales [keys, Hkv] lie far apart (a bound by max |v| of all keys would
+    hide what the small ones and the total lose).
+
+    With u = 2^-24, p the normalised weights, S = sum p |v| (per element) and P = 127 max p s_v:
+    scores are off by 48 u A as above, hence the weights by that share and 4 u, in the sum and
+    in the total: 2 (48 A + 4) u S. A weight is held to 2^-27 of the largest product (fixed point
+    of 31 bits whose reference is up to 32 times that product; f16 pairs: 2^-30), which is
+    L / 8 u P over all keys, and to 2^-23 of itself, 2 u S. f32 sums, flushes and truncating steps
+    stay below L / 2 + 32 roundings of S. f32 exponentials are zero below 2^-126 of their
+    reference, which is up to 2^4 above the row's largest weight (or the largest total of a part,
+    at least that weight): a key below 2^-120 of the largest weight may be missing, and its whole
+    share is allowed. Last, results below 2^-126 are multiples of 2^-149."""
+    n, H, d = q.shape
+    G = H // k.shape[1]
+    out = np.zeros((n, H, d))
+    bound = np.full((n, H, d), 2.0 ** -148)
+    lim = np.minimum(L, L - n + np.arange(n) + 1)
+    for t in np.nonzero(lim > 0)[0]:
+        for h in range(H):
+            K, V, sv = (x[:lim[t], h // G] for x in (k, v, v_scale))
+            x = q[t, h].astype(np.float64)
+            s = K @ x * scale
+            p = np.exp(s - s.max())
+            far = np.where(p < 2.0 ** -120, p, 0.0) / p.sum()
+            p /= p.sum()
+            out[t, h] = p @ V
+            bound[t, h] += far @ np.abs(V)
+            A = (np.abs(K) @ np.abs(x)).max() * abs(scale)
+            S, P = p @ np.abs(V), 127 * (p * sv).max()
+            bound[t, h] += 2.0 ** -24 * (2 * 48 * A + 64 + lim[t] / 2) * (S + P)
+    return out, bound
+
+
 def logits(x, repetition=1.0, frequency=0.0, presence=0.0, history=(), bias=(), mask=None):
     """One row x [V]: history a list of ids, bias a list of (id, value), mask [V] bool."""
     y = x.astype(np.float64)
