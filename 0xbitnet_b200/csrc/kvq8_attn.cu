@@ -404,20 +404,23 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
 #pragma unroll
         for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, shx(top, d));
         // only of the rows that need it: no row's bits depend on another's
-        if (mn != M || top > Vr || since >= kFlushSlices) flush(mn, top > Vr ? 32.0f * top : Vr);
+        if (mn != M || top > Vr || since >= kFlushSlices)
+          flush(mn, top > Vr ? fmaxf(32.0f * top, FLT_MIN) : Vr);  // 1 / Vr stays finite
       }
       uint32_t b[2][2];  // weights: [digits 0 1 / 2 3][block]
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const float svk = kb ? sv.y : sv.x;
         // a finite scale adds 0, a NaN one poisons the total
-        const float poison = svk - svk, f = svk * inv_vr * 2147483648.0f;
+        // p f <= 1, and where f is beyond f32's range p is 0 and the weight too (0 * inf: NaN, as
+        // a whole number 0)
+        const float poison = svk - svk, f = svk * inv_vr;
         uint32_t w[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const float p = seen[kb][hh] ? ex2(s[kb][hh] - M) : 0.0f;
           l += seen[kb][hh] ? p + poison : 0.0f;
-          w[hh] = __float2uint_rn(p * f);
+          w[hh] = __float2uint_rn(p * f * 2147483648.0f);
         }
         // this lane: two keys of query row qd; wanted: four keys of row grp / 2, and of their
         // digits grp % 2 and 2 + grp % 2. Even columns fetch digits 0 and 2 (y0), odd 1 and 3.

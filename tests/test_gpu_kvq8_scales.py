@@ -41,7 +41,8 @@ def run_planted(torch, rng, n, H, Hkv, log2w, v_scale, B=1):
         assert False, (b, at, got[(b, *at)], want[at], bound[at])
 
 
-ROWS = [(40, 4, 2), (130, 2, 1)]  # the pass for many query rows
+# few query rows (4, 8 and 16 to a tile), and many
+ROWS = [(1, 2, 2), (4, 4, 2), (9, 2, 1), (40, 4, 2), (130, 2, 1)]
 
 
 @pytest.mark.parametrize("n,H,Hkv", ROWS)
