@@ -142,7 +142,8 @@ class KVCacheQ8:
     @classmethod
     def wrap(cls, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor,
              v_scale: torch.Tensor) -> "KVCacheQ8":
-        """A cache over existing buffers (not copied)."""
+        """A cache over existing buffers (not copied). Scales that are no powers of two count as
+        they are, too; they have to be 0 or normal numbers above 0."""
         self = cls.__new__(cls)
         for t, name in ((k, "k"), (v, "v")):
             _check(t, name, torch.int8, k.get_device())

@@ -27,8 +27,9 @@
 // every value scale of the part lies within 2^32 of 2^lv0: its reference is T = R - lv0 then, and no
 // weight that counts is flushed (R <= max s f + lv0 + 26, so a score 60 below the largest still has
 // w >= 2^-118). From the first unit with a scale farther off, or with a block of zeros (whose keys
-// have weight but no product), the rest of the part is `far`: the total has exponentials and a
-// reference T of its own, moved like R but by the scores alone, and R goes by the other blocks.
+// have weight but no product) or a scale that is no power of two, the rest of the part is `far`:
+// the total has exponentials and a reference T of its own, moved like R but by the scores alone, R
+// goes by the blocks that are not zero, and the weights are multiplied by the scale's mantissa.
 // The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
 // unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 //
@@ -347,7 +348,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
           scl > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127)
                      : scl == 0.0f ? kNoExp : lv0;
       if (!far && __any_sync(0xffffffffu, lane >= 8 && lane < 16 && k0 + kQ8Block * (lane & 7) < cur.len &&
-                                              fabsf(lv_lane - lv0) > kNear)) {
+                                              (fabsf(lv_lane - lv0) > kNear ||
+                                               (scl > 0.0f && (__float_as_uint(scl) & 0x7FFFFFu))))) {
         far = true;
         lv0 = R == -INFINITY ? R : R - lv0;  // what l counts in
       }
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       float xo;
       if (!exchange(xr, &xo)) break;
       xr = fmaxf(xr, xo);
-      const bool grow = xr > R + 15.0f;
+      const bool grow = xr > R + (far ? 14.0f : 15.0f);  // a mantissa is below 2
       const float Rn = grow ? ceilf(xr) - 7.0f : R;
       const float corr = grow ? ex2(R - Rn) : 1.0f;
       const bool drain = part_u > 0 && part_u % kDrain == 0;
@@ -480,9 +482,12 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
           const float block = (sum[0] + sum[1]) + (sum[2] + sum[3]);
           if (decltype(clean)::value || (!far && 16 * b < seen)) l = fmaf(block, lf, l);
           if constexpr (!decltype(clean)::value) {
-            if (lv == kNoExp) {
+            if (far) {
+              const float sv = __shfl_sync(0xffffffffu, scl_now, 8 + b);
+              const float mantissa =
+                  sv > 0.0f ? __uint_as_float((__float_as_uint(sv) & 0x7FFFFFu) | 0x3F800000u) : 0.0f;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+              for (int i = 0; i < 16; ++i) w[i] = lv == kNoExp ? 0.0f : w[i] * mantissa;
             }
           }
 #pragma unroll

@@ -297,6 +297,8 @@ OBN_API int obn_attention_decode_rope_at(const float* qkv, void* k_cache, void* 
  * block p / 16 of its sequence and KV head. Scales are powers of two, 0 for a block of
  * zeros, NaN for a block that took a NaN or an infinity (what reads it gives NaN). Start
  * from zeroed buffers. Half the bytes of the binary16 cache of obn_rope_kv_append.
+ * Read-back and attention take buffers from elsewhere too: any scale that is 0 or a normal number
+ * above 0 counts as it is. Not specified: negative, subnormal and infinite scales.
  *
  * obn_rope_kv_append with that cache: qkv [B*n, (H + 2*Hkv) * head_dim] f32; token t of
  * sequence b sits at position pos + t, or pos_dev[b] + t when pos_dev (device, [B]) is not

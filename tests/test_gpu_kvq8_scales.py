@@ -121,3 +121,36 @@ def test_one_far_scale(n, H, Hkv, exp):
     for S, B in ((3000, 1), (1500, 30)):
         run_planted(torch, rng, n, H, Hkv, rng.integers(-20, 1, S),
                     np.full(-(-S // ref.BLOCK), 2.0 ** exp), B)
+
+
+def any_scales(torch, rng, B, S, Hkv, k_exp, v_exp):
+    """A cache whose scales are any numbers, no powers of two; its f64 values and value scales."""
+    att = importlib.import_module("0xbitnet_b200.attention")
+    nb = -(-S // ref.BLOCK)
+    c = att.KVCacheQ8(B, S, Hkv, D)
+    vals = []
+    for codes, scale, (lo, hi) in ((c.k, c.k_scale, k_exp), (c.v, c.v_scale, v_exp)):
+        cn = rng.integers(-127, 128, (B, S, Hkv, D)).astype(np.int8)
+        sn = np.exp2(rng.uniform(lo, hi, (B, nb, Hkv))).astype(np.float32)
+        codes.copy_(torch.from_numpy(cn))
+        scale.copy_(torch.from_numpy(sn))
+        vals.append(np.stack([ref.values(cn[b], sn[b]) for b in range(B)]))
+    wide = np.repeat(sn.astype(np.float64), ref.BLOCK, axis=1)[:, :S]
+    return c, vals[0], vals[1], wide
+
+
+@pytest.mark.parametrize("B,n,H,Hkv,S", [(1, 1, 5, 1, 500), (2, 4, 8, 2, 300), (1, 9, 4, 2, 900),
+                                         (1, 40, 4, 2, 300), (2, 130, 2, 1, 700), (30, 130, 2, 1, 900)])
+@pytest.mark.parametrize("v_exp", [(-8, -4), (-100, -90), (-60, 60), (-126, -118)])
+def test_scales_that_are_no_powers_of_two(B, n, H, Hkv, S, v_exp):
+    """Wrapped buffers may hold any scales: each pass takes them as they are."""
+    torch = need_cuda()
+    att = importlib.import_module("0xbitnet_b200.attention")
+    rng = np.random.default_rng(B + n + S)
+    c, k, v, wide = any_scales(torch, rng, B, S, Hkv, (-8, -4), v_exp)
+    q = rng.standard_normal((B * n, H * D)).astype(np.float32)
+    got = att.attention_q8(torch.from_numpy(q).cuda(), c, H, n, S).cpu().numpy()
+    for b in range(min(B, 3)):
+        want, bound = ref.attention_by_products(q.reshape(B, n, H, D)[b], k[b], v[b], wide[b], S, SCALE)
+        err = np.abs(got.reshape(B, n, H, D)[b] - want)
+        assert np.all(err <= bound), (b, (err / bound).max())
