@@ -1614,11 +1614,4 @@ cudaError_t launch_gemm_gather(const WeightView& W, const int8_t* q, const float
   return gemm_bn<256, 4, 1, false, kOutPeers>(W, q, s_x, qsum, n, nullptr, nullptr, order, s, go);
 }
 
-cudaError_t read_and_clear_dev_error_gemm(uint32_t* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_dev_error, sizeof(uint32_t));
-  if (e != cudaSuccess) return e;
-  const uint32_t zero = 0;
-  return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(uint32_t));
-}
-
 }  // namespace obn

@@ -544,11 +544,4 @@ cudaError_t launch_bitlinear_mma(const WeightView& W, const float* gamma, float 
   return fused_nt<24>(W, gamma, eps, x, n, y, kind, s);
 }
 
-cudaError_t read_and_clear_dev_error_mma(uint32_t* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_dev_error, sizeof(uint32_t));
-  if (e != cudaSuccess) return e;
-  const uint32_t zero = 0;
-  return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(uint32_t));
-}
-
 }  // namespace obn

@@ -17,6 +17,8 @@
 #include <cuda_fp16.h>
 
 #include <cstdlib>
+#include <vector>
+
 #include "layout.cuh"
 #include "obn_common.cuh"
 
@@ -1376,20 +1378,27 @@ cudaError_t launch_gemv(const WeightView& W, const int8_t* q, const float* s_x,
   return gemv_dispatch<false>(W, q, s_x, qsum, n, y, nullptr, order, s);
 }
 
-cudaError_t read_and_clear_dev_error_kernels(uint32_t* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_dev_error, sizeof(uint32_t));
-  if (e != cudaSuccess) return e;
-  const uint32_t zero = 0;
-  return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(uint32_t));
+namespace {
+std::vector<DevErrorReader>& dev_error_readers() {
+  static std::vector<DevErrorReader> all;
+  return all;
+}
+}  // namespace
+
+bool list_dev_error(DevErrorReader reader) {
+  dev_error_readers().push_back(reader);
+  return true;
 }
 
 cudaError_t read_and_clear_dev_error(uint32_t* out) {
-  uint32_t a = 0, b = 0, c = 0;
-  cudaError_t e = read_and_clear_dev_error_kernels(&a);
-  if (e == cudaSuccess) e = read_and_clear_dev_error_gemm(&b);
-  if (e == cudaSuccess) e = read_and_clear_dev_error_mma(&c);
-  *out = a ? a : b ? b : c;
-  return e;
+  *out = 0;
+  for (DevErrorReader read : dev_error_readers()) {
+    uint32_t word = 0;
+    const cudaError_t e = read(&word);
+    if (e != cudaSuccess) return e;
+    if (*out == 0) *out = word;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace obn

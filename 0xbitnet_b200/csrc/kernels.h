@@ -97,10 +97,8 @@ int num_sms_cached();
 // Raises a kernel's dynamic shared memory limit (once per kernel and device).
 cudaError_t ensure_smem(const void* fn, size_t bytes);
 
-// Device error words (one per translation unit): read and reset.
-cudaError_t read_and_clear_dev_error_kernels(uint32_t* out);
-cudaError_t read_and_clear_dev_error_gemm(uint32_t* out);
-cudaError_t read_and_clear_dev_error_mma(uint32_t* out);
+// Device error words of all translation units (obn_common.cuh): read and reset; out takes the
+// first one that is set.
 cudaError_t read_and_clear_dev_error(uint32_t* out);
 
 }  // namespace obn

@@ -22,8 +22,20 @@ enum : uint32_t {
   DEVERR_BAD_LAUNCH = 2,  // launch geometry outside what the kernel was built for
 };
 // Internal linkage: every translation unit (built without -rdc) owns its own
-// copy and exposes it through a host reader (kernels.h).
+// copy, and lists a reader of it as the library is loaded, so that
+// read_and_clear_dev_error (kernels.h) knows them all.
 static __device__ uint32_t g_dev_error = 0;
+
+using DevErrorReader = cudaError_t (*)(uint32_t* out);
+bool list_dev_error(DevErrorReader reader);  // kernels.cu
+static cudaError_t read_and_clear_own_dev_error(uint32_t* out) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_dev_error, sizeof(uint32_t));
+  if (e != cudaSuccess || *out == 0) return e;
+  const uint32_t zero = 0;
+  return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(uint32_t));
+}
+[[maybe_unused]] static const bool g_dev_error_listed =
+    list_dev_error(&read_and_clear_own_dev_error);
 
 // Spin bound for mbarrier waits. try_wait suspends the thread for a
 // hardware-chosen interval per attempt, so this bounds the wait at well under
