@@ -597,6 +597,30 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       }
       cur = nxt;
     }
+    // After an abort: NaN for the rows that this warp would have written (a part's sums, or outputs),
+    // of this pair and of the share's others, so that nothing stale passes for a result.
+    while (cur.left > 0) {
+      Q8Cursor nxt = cur;
+      q8_next(sc, nxt);
+      const bool pair_ends = cur.unit + 1 == cur.units;
+      if (pair_ends || nxt.left == 0) {
+        const float nan = __int_as_float(0x7FC00000);
+        const int slot = 2 * blockIdx.x + (u_first == 0 ? 1 : 0);
+        const int row0 = 128 * x + 16 * (warp & 7);
+#pragma unroll 1
+        for (int i = row0; i < row0 + 16; ++i) {
+          const int qr = cur.tile * kRows + i, t = qr / sc.G;
+          if (qr >= rows_seq) break;
+          float* dst = pair_ends && u_first == 0
+                           ? out + ((static_cast<size_t>(cur.b) * sc.n + t) * H + cur.kvh * sc.G +
+                                    (qr - t * sc.G)) * D
+                           : q8_part_o(ws, kRows, slot) + static_cast<size_t>(i) * D;
+          *reinterpret_cast<float4*>(dst + 4 * lane) = make_float4(nan, nan, nan, nan);
+        }
+        u_first = 0;
+      }
+      cur = nxt;
+    }
   } else if (warp < 20) {
     // ---- codes to f16 ------------------------------------------------------------------------
     const int ct = tid - 512, cw = ct >> 5;

@@ -54,3 +54,14 @@ def test_the_check_reads_every_listed_word():
                      text("kernels.cu"), re.S)[1]
     assert re.search(r"for \(DevErrorReader (\w+) : dev_error_readers\(\)\)", body)
     assert "read_and_clear_dev_error(&word)" in text("abi.cu")
+
+
+def test_an_aborted_share_of_many_rows_leaves_nan():
+    """After the softmax loop, which a wait that gives up leaves before the share is done, each
+    warp fills the rows that are its own to write, to the end of the share."""
+    src = text("kvq8_many.cu")
+    after = src[src.index("for (int u = 0; cur.left > 0; ++u)"):src.index("} else if (warp < 20)")]
+    fill = re.search(r"\n    \}\s*while \(cur\.left > 0\) \{(.*)", after, re.S)[1]
+    assert "q8_next(sc, nxt)" in fill and "cur = nxt;" in fill
+    assert re.search(r"i < row0 \+ 16;", fill) and "make_float4(nan, nan, nan, nan)" in fill
+    assert "q8_part_o(ws, kRows, slot)" in fill and "out +" in fill
