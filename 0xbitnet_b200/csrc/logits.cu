@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
   const int step = cluster * kSliceIds;
   const int own = 4 * tid - mis;  // the thread's first id in a slice, from the slice's position
   const int sh = own & 31;        // its bit in a mask word: slices are whole words
-  bool dead = false;  // a copy did not come in time: no more of them
+  bool dead = false;  // a copy did not come in time
 
   // Quads [q_head, q_end) of the slice at p0 lie in the row; one before them and one behind may
   // be cut by the row's ends.
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
   auto request = [&](int p0, int buf) {
     const int cnt = min(kSliceIds, end - p0), nq = (cnt + 3) / 4;
     const int head = q_head(p0), whole = q_end(p0) - head;
-    if (tid == 0 && whole > 0 && !dead) {
+    if (tid == 0 && whole > 0) {
       fence_proxy_async_smem();  // threads read and wrote the buffer before
       mbar_arrive_expect_tx(&sm.full[buf], whole * 16);
       bulk_g2s(&sm.x[buf][4 * head], x_row + (p0 + 4 * head - mis), whole * 16, &sm.full[buf]);
@@ -185,8 +185,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
   float best = -INFINITY;
   int best_at = 0;
   uint32_t phase = 0;
-  int buf = 0;
-  for (int p0 = p_first; p0 < end; p0 += step, buf ^= 1) {
+  int buf = 0, p0 = p_first;
+  for (; p0 < end; p0 += step, buf ^= 1) {
     const int cnt = min(kSliceIds, end - p0), nq = (cnt + 3) / 4;
     const bool wait = copied;
     if (p0 + step < end) copied = request(p0 + step, buf ^ 1);
@@ -237,9 +237,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
       }
     }
     float* x = sm.x[buf];
-    if (wait && !dead) dead = !mbar_wait(&sm.full[buf], (phase >> buf) & 1);
+    dead = __syncthreads_or(wait && !mbar_wait(&sm.full[buf], (phase >> buf) & 1));
+    if (dead) break;
     if (wait) phase ^= 1u << buf;
-    __syncthreads();
     // 2. rewrite
     const int founds = hist ? sm.founds : 0;
     for (int i = tid; i < founds; i += kThreads) {
@@ -329,6 +329,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
     }
   }
 
+  if (dead) {  // nothing of the slice was used: NaN for the rest of the CTA's ids, and no token
+    if (tid == 0) {  // the copies may still be on their way into this CTA's shared memory
+      mbar_wait(&sm.full[buf], (phase >> buf) & 1);
+      if (copied && p0 + step < end) mbar_wait(&sm.full[buf ^ 1], (phase >> (buf ^ 1)) & 1);
+    }
+    for (; p0 < end; p0 += step)
+      for (int p = max(p0, mis) + tid; p < min(p0 + kSliceIds, end); p += kThreads)
+        y_row[p - mis] = __int_as_float(0x7FC00000);
+  }
+
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (!token) return;
   // the largest key, and the lowest id that has it
@@ -340,7 +350,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_logits(const float* logits, int
       if (v >= 0 && v < V && y_row[v] == best) at = v;
     }
   }
-  const uint32_t mine = best > -INFINITY ? key_of(best) : 0u;  // 0: nothing above -inf
+  // 0: nothing above -inf; no float has all bits of a key set, and the token is -1 with that one
+  if (dead) at = 0xFFFFFFFFu;
+  const uint32_t mine = dead ? 0xFFFFFFFFu : best > -INFINITY ? key_of(best) : 0u;
   const uint32_t wk = __reduce_max_sync(0xffffffffu, mine);
   const uint32_t wa = __reduce_min_sync(0xffffffffu, mine == wk ? at : 0xFFFFFFFFu);
   if (lane == 0) {

@@ -65,3 +65,15 @@ def test_an_aborted_share_of_many_rows_leaves_nan():
     assert "q8_next(sc, nxt)" in fill and "cur = nxt;" in fill
     assert re.search(r"i < row0 \+ 16;", fill) and "make_float4(nan, nan, nan, nan)" in fill
     assert "q8_part_o(ws, kRows, slot)" in fill and "out +" in fill
+
+
+def test_a_late_copy_of_logits_leaves_nan_and_no_token():
+    """The block agrees on a copy that did not come, uses nothing of it, waits for what is in
+    flight, fills the rest with NaN and lets no other block's maximum win."""
+    src = text("logits.cu")
+    assert re.search(r"dead = __syncthreads_or\(wait && !mbar_wait\(&sm\.full\[buf\][^;]*;\s*"
+                     r"if \(dead\) break;", src)
+    late = src[src.index("if (dead) {"):src.index("if (!token) return;")]
+    assert late.count("mbar_wait(&sm.full[") == 2
+    assert re.search(r"y_row\[p - mis\] = __int_as_float\(0x7FC00000\);", late)
+    assert "mine = dead ? 0xFFFFFFFFu" in src
