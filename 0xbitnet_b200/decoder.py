@@ -176,6 +176,10 @@ class BitNetDecoder:
                     B, 1, H, d, ctx))), dtype=torch.uint8, device=dev)
             else:
                 self.attn_ws = att.attention_q8_workspace(self.caches[0], H, 1)
+                # positions with the last step's token, 0 for a sequence without one; and
+                # whether that step's positions were on the device
+                self.lengths = torch.ones((B,), dtype=torch.int32, device=dev)
+                self._ragged = False
             self.logits = torch.empty((B, cfg.vocab), **f32)
             self.lm_ws = torch.empty(max(1, int(lib().obn_lm_head_workspace_bytes(B, D))),
                                      dtype=torch.uint8, device=dev)
@@ -202,10 +206,22 @@ class BitNetDecoder:
                                   self.B, _ptr(self.x), s))
 
     def _lengths(self, pos):
-        """The sequences' lengths with the step's token, as the attention takes them."""
-        if self.kv_bits == 16 and isinstance(pos, torch.Tensor):
-            raise TypeError("positions per sequence need the 8-bit cache (kv_bits=8)")
-        return pos + 1
+        """The sequences' lengths with the step's token, as the attention takes them.
+        Positions on the device are not checked: one outside the cache has no token."""
+        ragged = isinstance(pos, torch.Tensor)
+        if self.kv_bits == 16:
+            if ragged:
+                raise TypeError("positions per sequence need the 8-bit cache (kv_bits=8)")
+            return pos + 1
+        if not ragged:
+            if self._ragged:
+                self.lengths.fill_(1)
+            self._ragged = False
+            return pos + 1
+        att._check(pos, "pos", torch.int32, self.lengths.get_device(), self.B)
+        self._ragged = True
+        torch.add(pos.view(-1), 1, out=self.lengths)
+        return self.lengths.masked_fill_(self.lengths > self.ctx, 0)
 
     def _layer(self, L, c, pos, lengths) -> None:
         """One transformer block on self.x in place (transformer.rs:51-72)."""
@@ -237,7 +253,9 @@ class BitNetDecoder:
         """Enqueues one decode step for the tokens in self.ids at position `pos`
         (every cache holds pos positions before it); returns logits [B, vocab].
         With 8-bit caches pos may be an int32 tensor [B] on the device: a position
-        for each sequence (-1: an idle one, whose cache stays as it is)."""
+        for each sequence. One whose position is outside [0, ctx) takes no part (-1: an
+        idle one; ctx: one that is full): its cache stays as it is, its logits mean
+        nothing, and pick() gives -1 for it."""
         lengths = self._lengths(pos)
         self._embed(_stream(self.device))
         for L, c in zip(self.layers, self.caches):
@@ -246,8 +264,11 @@ class BitNetDecoder:
 
     def pick(self, logits: torch.Tensor, rules: LogitRules) -> torch.Tensor:
         """Applies the rules to the logits in place and leaves each sequence's
-        greedy token (-1: nothing allowed) in self.ids for the next step."""
+        greedy token (-1: nothing allowed, or no token in the step) in self.ids for the
+        next step."""
         logits_process(logits, rules, out=logits, token=self.ids)
+        if self.kv_bits == 8 and self._ragged:
+            self.ids.masked_fill_(self.lengths <= 0, -1)
         return self.ids
 
     def diagnose(self, pos: int | torch.Tensor) -> list[dict]:
