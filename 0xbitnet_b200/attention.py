@@ -192,7 +192,8 @@ def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
     [B*n, H*d]; token t of sequence b is stored at position pos + t (pos[b] + t for an int32
     tensor [B] on the device; cache.seq_len by default). Tokens whose position is outside
     the cache are not stored and get a zero q row when pos is a tensor, and are refused when
-    it is an int."""
+    it is an int, after which cache.seq_len is pos + n or more: calls without pos append one
+    behind the other. Positions on the device leave cache.seq_len as it is."""
     B, Hkv, d = cache.B, cache.Hkv, cache.head_dim
     _check(qkv, "qkv", torch.float32, cache.index, B * n * (H + 2 * Hkv) * d)
     if q_out is None:
@@ -203,6 +204,8 @@ def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
     _call("obn_rope_kv_append_q8", cache.index, qkv.data_ptr(), B, n, H, Hkv, d, host, dev,
           theta_base, q_out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
           cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.S_max)
+    if dev is None:
+        cache.seq_len = max(cache.seq_len, host + n)
     return q_out
 
 
