@@ -99,8 +99,11 @@ def attention_rope(qkv: torch.Tensor, cache: KVCache, H: int, pos: int,
 Q8_BLOCK = 16  # positions that share a scale
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle, without a Stream object
-_current_device = torch._C._cuda_getDevice
+# The current stream's handle without a Stream object, and the current device, where torch has
+# these calls (its CUDA builds do): a decode step makes two such calls a layer.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(name: str, index: int, *args) -> None:
