@@ -41,3 +41,36 @@ def test_appends_without_a_position_follow_one_another():
     with pytest.raises(importlib.import_module("0xbitnet_b200").ObnError):
         att().rope_kv_append_q8(rows(qkv[:, :2 * n - 1]), two, H, 2 * n - 1)  # no room for all
     assert two.seq_len == 2 * n
+
+
+@pytest.mark.parametrize("B,n,H,Hkv,S,ragged", [
+    (1, 4, 300, 75, 6000, False), (2, 4, 320, 80, 2000, False), (4, 4, 160, 40, 1000, False),
+    (8, 1, 40, 40, 3000, False), (1, 1, 32, 32, 60000, False), (3, 4, 128, 32, 2000, True),
+    (1, 2, 150, 150, 5000, True), (1, 1, 300, 300, 3000, False)])
+def test_many_kv_heads(B, n, H, Hkv, S, ragged):
+    """KV heads that do not divide the CTAs, few of them and more than there are CTAs: every head
+    and sequence against the same call for that head alone (another split of the keys)."""
+    torch = need_cuda()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(B + Hkv)
+    c = att().KVCacheQ8(B, S, Hkv)
+    for t in (c.k, c.v):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=g, device="cuda").to(torch.int8))
+    for t in (c.k_scale, c.v_scale):
+        t.copy_(torch.exp2(torch.randint(-8, -4, t.shape, generator=g, device="cuda").float()))
+    q = torch.randn((B, n, H, D), generator=g, device="cuda")
+    L = [S - 700 * b for b in range(B)] if ragged else [S] * B
+    arg = torch.tensor(L, dtype=torch.int32, device="cuda") if ragged else S
+    got = att().attention_q8(q.view(B * n, -1), c, H, n, arg).view(B, n, H, D)
+    G = H // Hkv
+    for h in sorted({0, 1, Hkv // 2, Hkv - 2, Hkv - 1}):
+        for b in range(B):
+            one = att().KVCacheQ8.wrap(*[t[b:b + 1, :, h:h + 1].contiguous()
+                                         for t in (c.k, c.k_scale, c.v, c.v_scale)])
+            rows = q[b, :, h * G:(h + 1) * G].reshape(n, -1).contiguous()
+            want = att().attention_q8(rows, one, G, n, L[b]).view(n, G, D)
+            # both are f32 results of the same values: apart by two roundings of the scores' range
+            # (|s| < 64 in log2, 48 u of it and of the sums' 24 steps), relative to the mean of |v|
+            err = (got[b, :, h * G:(h + 1) * G] - want).abs().max().item()
+            top = (one.v.float().abs().amax() * one.v_scale.max()).item()
+            assert err <= 2 * 2.0 ** -24 * (2 * 48 * 64 + 64) * top, (h, b, err)
