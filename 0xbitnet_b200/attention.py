@@ -185,7 +185,15 @@ def _host_or_dev(value, cache: KVCacheQ8, name: str) -> tuple[int, int | None]:
     if isinstance(value, torch.Tensor):
         _check(value, name, torch.int32, cache.index, cache.B)
         return 0, value.data_ptr()
-    return int(value), None
+    return _int32(value, name), None
+
+
+def _int32(value, name: str) -> int:
+    """An int that the C ABI takes as it is: ctypes would drop the upper bits of a larger one."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} = {value} is no 32-bit number")
+    return value
 
 
 def rope_kv_append_q8(qkv: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
@@ -241,7 +249,7 @@ def attention_q8(q: torch.Tensor, cache: KVCacheQ8, H: int, n: int,
         _check(workspace, "workspace", torch.uint8, cache.index)
     host, dev = _host_or_dev(seq_len, cache, "seq_len")
     if dev is not None:
-        host = cache.S_max if max_len is None else max_len
+        host = cache.S_max if max_len is None else _int32(max_len, "max_len")
     _call("obn_attention_q8", cache.index, q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
           cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), B, n, H, Hkv, d, cache.S_max, host,
           dev, d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
