@@ -48,6 +48,8 @@ class LogitRules:
         s.bias_values = self._list(bias_values, "bias_values", torch.float32)[0]
         s.bias_lens = self._vector(bias_lens, "bias_lens", torch.int32)
         s.mask, s.mask_ld, self.mask_words = self._list(mask, "mask", torch.int32)
+        if mask is not None and not self.mask_words:
+            raise ValueError("mask holds no words")
 
     def _take(self, t, name, dtype):
         if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype
@@ -76,10 +78,10 @@ class LogitRules:
         if t is None:
             return None, 0, 0
         self._take(t, name, dtype)
+        if t.dim() not in (1, 2):
+            raise ValueError(f"{name} must be [rows, cap] or [cap]")
         if t.dim() == 1 or t.shape[0] == 1:
             return t.data_ptr(), 0, t.shape[-1]
-        if t.dim() != 2:
-            raise ValueError(f"{name} must be [rows, cap] or [cap]")
         self._agree(t.shape[0], name)
         return t.data_ptr(), t.shape[1], t.shape[1]
 

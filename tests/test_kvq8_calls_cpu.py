@@ -37,3 +37,33 @@ def test_positions_beyond_32_bits_are_refused(value):
         att._host_or_dev(value, None, "pos")
     assert att._host_or_dev(2 ** 31 - 1, None, "pos") == (2 ** 31 - 1, None)
     assert att._host_or_dev(-2 ** 31, None, "pos") == (-2 ** 31, None)
+
+
+def cpu_rules(**kw):
+    """LogitRules of tensors on the CPU: its own checks but for the device's; nothing is launched."""
+    import torch
+    lg = importlib.import_module("0xbitnet_b200.logits")
+
+    class Rules(lg.LogitRules):
+        def _take(self, t, name, dtype):
+            assert t.dtype is dtype
+            self._kept.append(t)
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    return Rules(**{k: i32(*v) if k != "bias_values" else torch.zeros(v) for k, v in kw.items()})
+
+
+@pytest.mark.parametrize("shapes", [
+    dict(mask=(4, 0)), dict(mask=(0,)), dict(mask=(1, 0)),            # an empty mask allowed all ids
+    dict(history=(1, 3, 5)), dict(mask=(1, 2, 4)), dict(history=()),  # only [rows, cap] or [cap]
+    dict(bias_ids=(1, 2, 2), bias_values=(1, 2, 2)), dict(history=(2, 3, 5))])
+def test_rule_lists_of_other_shapes_are_refused(shapes):
+    with pytest.raises(ValueError):
+        cpu_rules(**shapes)
+
+
+def test_rule_lists_that_stay_allowed():
+    assert cpu_rules(mask=(3, 4)).mask_words == 4
+    r = cpu_rules(history=(1, 7), mask=(5,))
+    assert (r._struct.history_ld, r._struct.history_cap, r.rows) == (0, 7, None)
+    r = cpu_rules(history=(2, 0), bias_ids=(2, 3), bias_values=(2, 3))
+    assert (r._struct.history_cap, r._struct.bias_cap, r.rows) == (0, 3, 2)
