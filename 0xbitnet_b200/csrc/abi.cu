@@ -1028,6 +1028,10 @@ int obn_logits_process(const float* logits, int rows, int vocab, const obn_logit
                         static_cast<const void*>(rules->bias_values),
                         static_cast<const void*>(rules->bias_lens)})
     if (!aligned(p, 4)) return fail(OBN_ERR_INVALID_ARGUMENT, "pointers must be 4-byte aligned");
+  const uintptr_t in = reinterpret_cast<uintptr_t>(logits), to = reinterpret_cast<uintptr_t>(out);
+  const uintptr_t bytes = static_cast<uintptr_t>(rows) * static_cast<uintptr_t>(vocab) * sizeof(float);
+  if (in != to && in < to + bytes && to < in + bytes)
+    return fail(OBN_ERR_INVALID_ARGUMENT, "out may be logits itself, but not overlap it otherwise");
   cudaError_t e = obn::launch_logits_process(logits, rows, vocab, *rules, out, token,
                                              static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "logit rules launch");

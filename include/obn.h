@@ -376,7 +376,7 @@ typedef struct obn_logit_rules {
 
 /* out[r, v] = the logits [rows, vocab] under the rules, in the order above: repetition,
  * frequency and presence, biases, mask; a changed value is computed in f64 and rounded once,
- * the others pass unchanged. out may be logits itself. token (nullable, [rows]) takes each
+ * the others pass unchanged. out may be logits itself (no other overlap). token (nullable, [rows]) takes each
  * row's greedy choice: the largest out[r, v], the lowest v among equals, NaN never; -1 when
  * nothing is above -inf. A single occurrence gives the bits of the sampler's own penalty. */
 OBN_API int obn_logits_process(const float* logits, int rows, int vocab,

@@ -67,3 +67,14 @@ def test_rule_lists_that_stay_allowed():
     assert (r._struct.history_ld, r._struct.history_cap, r.rows) == (0, 7, None)
     r = cpu_rules(history=(2, 0), bias_ids=(2, 3), bias_values=(2, 3))
     assert (r._struct.history_cap, r._struct.bias_cap, r.rows) == (0, 3, 2)
+
+
+@pytest.mark.parametrize("shift", [4, -4, 4 * 100, 4 * 199, -4 * 199])
+def test_overlapping_logits_and_out_are_refused(shift):
+    """Rows written over others that are still to be read; refused before anything is launched."""
+    import ctypes
+    obn = importlib.import_module("0xbitnet_b200")
+    rules = obn._lib.LogitRulesStruct()
+    at = 1 << 20  # never read
+    assert obn.lib().obn_logits_process(at, 2, 100, ctypes.addressof(rules), at + shift, None, None) == -1
+    assert b"overlap" in obn.lib().obn_error_message()
