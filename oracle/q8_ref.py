@@ -133,6 +133,35 @@ def attention_by_products(q, k, v, v_scale, L, scale):
     return out, bound
 
 
+def attention_rms(q, k, v, L, scale):
+    """attention() with, for each row [n, H], how large the error's root mean square over the row's
+    d elements may be: near what f32 arithmetic leaves, so that a weight or query held in one
+    f16, or one key too many or too few, shows (a key of average weight is 1 / sqrt(L) of the
+    output's root mean square).
+
+    u = 2^-24. A weight is off by ln 2 times the error of its score in base 2, s, whose roundings are
+    2 u of the factor, u of the product, 2 u of q's halves, and at most 2 u of what is added up in
+    each of 16 truncating tensor core steps: 37 u |s| ln 2 < 26 u |s| in all; and by 4 u of the
+    exponential. Errors of keys are independent, as the values are, so their root mean square in
+    the output is that of the weights' relative errors (weighted by p^2) times the output's.
+    Sums of O are off by a bias of 2.5 u a unit for up to 3 units, by one rounding a flush, part
+    or join, and the total by as much: 24 u. Twice that for the spread of a row's 128 elements."""
+    n, H, d = q.shape
+    G = H // k.shape[1]
+    out, tol = np.zeros((n, H, d)), np.zeros((n, H))
+    lim = np.minimum(L, L - n + np.arange(n) + 1)
+    hidden = np.arange(L)[None] >= lim[:, None]
+    for h in range(H):
+        K, V, Q = k[:L, h // G], v[:L, h // G], q[:, h].astype(np.float64)
+        s = np.where(hidden, -np.inf, Q @ K.T * scale)
+        p = np.exp(s - s.max(1, keepdims=True))
+        out[:, h] = p @ V / p.sum(1, keepdims=True)
+        s = np.where(hidden, 0.0, s) / np.log(2.0)
+        rms = np.sqrt((p * p * s * s).sum(1) / (p * p).sum(1))
+        tol[:, h] = 2 * 2.0 ** -24 * (26 * rms + 4 + 24) * np.sqrt((out[:, h] ** 2).mean(-1))
+    return out, tol
+
+
 def logits(x, repetition=1.0, frequency=0.0, presence=0.0, history=(), bias=(), mask=None):
     """One row x [V]: history a list of ids, bias a list of (id, value), mask [V] bool."""
     y = x.astype(np.float64)

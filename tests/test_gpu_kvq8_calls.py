@@ -74,3 +74,27 @@ def test_many_kv_heads(B, n, H, Hkv, S, ragged):
             err = (got[b, :, h * G:(h + 1) * G] - want).abs().max().item()
             top = (one.v.float().abs().amax() * one.v_scale.max()).item()
             assert err <= 2 * 2.0 ** -24 * (2 * 48 * 64 + 64) * top, (h, b, err)
+
+
+@pytest.mark.parametrize("R,V", [(1, 40000), (3, 9999), (5, 31), (2, 1), (64, 1003)])
+@pytest.mark.parametrize("x_off,y_off", [(0, 1), (1, 0), (2, 1), (3, 3), (1, 2)])
+def test_logits_and_out_of_different_alignment(R, V, x_off, y_off):
+    """Buffers that begin 0 to 3 elements behind a 16-byte boundary: the same bits, and nothing
+    around the output is written."""
+    torch = need_cuda()
+    lg = importlib.import_module("0xbitnet_b200.logits")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(R + V)
+    x = torch.randn((R, V), generator=g, device="cuda")
+    hist = torch.randint(0, V, (R, 200), generator=g, device="cuda").int()
+    mask = torch.randint(-2 ** 31, 2 ** 31 - 1, (R, -(-V // 32)), generator=g, device="cuda").int()
+    ids = torch.randint(0, V, (R, 9), generator=g, device="cuda").int()
+    rules = lg.LogitRules(repetition=torch.full((R,), 1.3, device="cuda"), history=hist, mask=mask,
+                          bias_ids=ids, bias_values=torch.randn((R, 9), generator=g, device="cuda"))
+    want, token = lg.logits_process(x, rules)
+    a, b = torch.full((2, R * V + 8), 5.0, device="cuda")
+    a[x_off:x_off + R * V] = x.view(-1)
+    out = b[y_off:y_off + R * V].view(R, V)
+    _, got = lg.logits_process(a[x_off:x_off + R * V].view(R, V), rules, out=out)
+    assert torch.equal(out, want) and torch.equal(got, token)
+    assert bool((b[:y_off] == 5.0).all()) and bool((b[y_off + R * V:] == 5.0).all())

@@ -78,3 +78,26 @@ def test_overlapping_logits_and_out_are_refused(shift):
     at = 1 << 20  # never read
     assert obn.lib().obn_logits_process(at, 2, 100, ctypes.addressof(rules), at + shift, None, None) == -1
     assert b"overlap" in obn.lib().obn_error_message()
+
+
+def test_a_call_runs_on_its_tensors_device(monkeypatch):
+    """From another current device: the device is switched for the call, and the stream is that
+    device's. From the same one: no switch."""
+    import contextlib
+    import types
+    att = importlib.import_module("0xbitnet_b200.attention")
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(index):
+        was, current[0] = current[0], index
+        yield
+        current[0] = was
+    entry = lambda *args: seen.append((current[0], args)) or 0
+    monkeypatch.setattr(att, "lib", lambda: types.SimpleNamespace(obn_entry=entry))
+    monkeypatch.setattr(att, "_current_device", lambda: current[0])
+    monkeypatch.setattr(att, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(att.torch.cuda, "device", device)
+    att._call("obn_entry", 1, "a", 2)
+    att._call("obn_entry", 0, "b")
+    assert seen == [(1, ("a", 2, 101)), (0, ("b", 100))] and current == [0]
