@@ -33,12 +33,13 @@
 // The tensor cores truncate when they add to an accumulator, a bias of 1.5e-7 of O for every
 // unit: after kDrain units O moves to an f32 copy in the workspace (L2) and starts anew.
 //
-// 2048 tokens of 20/5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 222 us,
-// 0.48 PFLOP/s, 0.97 with the low halves. A unit takes about 9100 cycles, its products 5200: a tile's
-// scores and weights share tensor memory, so its softmax (maximum 900, exchange 600, weights
-// 2700, copies 1100 cycles) and its products (2600) follow one another, and the other tile's
-// products fill only half of the softmax. 512 rows over 2100 keys: 47 us; a pair's query rows and
-// its output cost 8000 cycles each there, as much as two of the three units that a CTA has.
+// 2048 tokens of 20/5 heads over 6144 keys (107 GFLOP, twice that with the low halves): 252 us from
+// cold caches, the join among them, 0.43 PFLOP/s, 0.85 with the low halves (244 us before far scales
+// had code). A unit takes about 9100 cycles (taken when a call took 222 us with a warm L2), its
+// products 5200: a tile's scores and weights share tensor memory, so its softmax (maximum 900,
+// exchange 600, weights 2700, copies 1100 cycles) and its products (2600) follow one another, and
+// the other tile's products fill only half of the softmax. 512 rows over 2100 keys: 47 us; a pair's
+// query rows and its output cost 8000 cycles each there, as much as two of a CTA's three units.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -58,8 +59,9 @@ constexpr int D = kQ8HeadDim;
 constexpr int kRows = 256;       // query rows of a CTA's pair of tiles
 constexpr int kThreads = 672;
 // Units between O's moves to its copy. Error against 64 bits (512 rows over 2100 keys, 2048 over
-// 6144) and time of the latter: 2 units 1.3e-6, 1.4e-6, 236 us; 3: 1.5e-6, 1.6e-6, 227 us (222 now); 4: 1.7e-6,
-// 1.9e-6, 219 us; 8: 2.9e-6. An f32 softmax and product of the same values: 1.2e-6, 1.7e-6.
+// 6144) and time of the latter with a warm L2, when this was chosen: 2 units 1.3e-6, 1.4e-6, 236 us;
+// 3: 1.5e-6, 1.6e-6, 227 us; 4: 1.7e-6, 1.9e-6, 219 us; 8: 2.9e-6. An f32 softmax and product of the
+// same values: 1.3e-6, 1.7e-6, so 512 rows are a little above it and 2048 a little below.
 constexpr int kDrain = 3;
 constexpr float kNear = 32.0f;  // how far from lv0 a value scale's exponent may be
 constexpr float kNoExp = -1000.0f;  // the exponent of a scale of zero
@@ -147,8 +149,8 @@ OBN_DEVINL void bytes_to_half(uint32_t w, uint32_t* h01, uint32_t* h23) {
   *h23 = *reinterpret_cast<uint32_t*>(&hb);
 }
 
-// q8_wait of the MMA warp, without sleep: it is one warp, and every product waits for it (2048 tokens
-// 227 -> 222 us; softmax warps that spin as well take the slots of those that work: 231 us).
+// q8_wait of the MMA warp, without sleep: it is one warp, and every product waits for it (2048 tokens,
+// warm, 227 -> 222 us; softmax warps that spin as well take the slots of those that work: 231 us).
 OBN_DEVINL bool mma_wait(volatile int* abort_flag, uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 24); ++i) {
     uint32_t ok;
@@ -347,9 +349,9 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_q8_many(
       const float lv_lane =
           scl > 0.0f ? static_cast<float>(static_cast<int>(__float_as_uint(scl) >> 23) - 127)
                      : scl == 0.0f ? kNoExp : lv0;
-      if (!far && __any_sync(0xffffffffu, lane >= 8 && lane < 16 && k0 + kQ8Block * (lane & 7) < cur.len &&
-                                              (fabsf(lv_lane - lv0) > kNear ||
-                                               (scl > 0.0f && (__float_as_uint(scl) & 0x7FFFFFu))))) {
+      const bool held = lane >= 8 && lane < 16 && k0 + kQ8Block * (lane & 7) < cur.len;
+      const bool mantissa = scl > 0.0f && (__float_as_uint(scl) & 0x7FFFFFu);
+      if (!far && __any_sync(0xffffffffu, held && (fabsf(lv_lane - lv0) > kNear || mantissa))) {
         far = true;
         lv0 = R == -INFINITY ? R : R - lv0;  // what l counts in
       }

@@ -223,7 +223,6 @@ OBN_DEVINL void q8_next(const Q8Sched& s, Q8Cursor& c) {
 }
 
 OBN_DEVINL float shx(float v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
-OBN_DEVINL uint32_t shxu(uint32_t v, int m) { return __shfl_xor_sync(0xffffffffu, v, m); }
 OBN_DEVINL float ex2(float x) {  // 2^x; results below 2^-126 become 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

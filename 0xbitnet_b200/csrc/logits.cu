@@ -15,12 +15,13 @@
 //   2. the list's logits are rewritten in place, in f64, rounded once; an id with a bias is left
 //      to the first of its bias entries, which has the sum of all of them in list order
 //   3. the slice streams out, with the mask and the row's maximum
-// With the list the f64 work falls on full warps. Histories crowd in a few slices and are
-// sparse in the others: 64 rows of 128256 with 4096 ids took 123 us when the threads that stream
-// the logits rewrote them in passing, 38 us when the threads that count an id rewrote it,
-// 58 us with the history spread over the cluster and remote counters, 40 us when the marked ids were
-// gathered and the others streamed through registers past them, without staging; 30 us as it is, 16
-// without any rule. Three smaller slices on their way took 37 us, twice the CTAs 35 us.
+// With the list the f64 work falls on full warps. Histories crowd in a few slices and are sparse in
+// the others: 64 rows of 128256 with 4096 ids took 123 us when the threads that stream the logits
+// rewrote them in passing, 38 us when the threads that count an id rewrote it, 58 us with the
+// history spread over the cluster and remote counters, 40 us when the marked ids were gathered and
+// the others streamed through registers past them, without staging; 30 us as it is, 14 without any
+// rule (the kernel from cold caches). Three smaller slices on their way took 37 us, twice the CTAs
+// 35 us.
 #include "logits.h"
 
 #include <cmath>

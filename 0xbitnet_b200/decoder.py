@@ -26,7 +26,8 @@ accumulation) instead of the shader-order one. Weights are random (seeded)
 with the reference's distributions; no checkpoint is needed to measure speed.
 
 With kv_bits=8 the caches are held in 8 bits (half the bytes, so twice the
-context or sequences), and the sequences may be at positions of their own. pick()
+context or sequences; 64 sequences decode 1.3 to 1.6 times as fast at contexts of
+2048 and 4096, one alone 0.84 times), and the sequences may be at positions of their own. pick()
 applies logit rules and leaves each sequence's greedy token as the next step's
 input, so a whole decode iteration is one captured graph without a host read.
 """

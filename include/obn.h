@@ -311,6 +311,8 @@ OBN_API int obn_attention_decode_rope_at(const float* qkv, void* k_cache, void* 
  * A block's rows requantize only when its scale grows, which at least doubles it, so a held
  * value is within s of the appended one (s / 2 if nothing larger came later). Rows of the
  * block behind the appended ones keep their codes and lose their meaning: append in order.
+ * Magnitudes above 2^127 may read back as infinities. q is rotated in f32 (three roundings of
+ * 2^-24), k in f64.
  * A token whose position is outside [0, S_max) is stored nowhere and gets a zero q row (left
  * padding and idle sequences: a negative pos_dev[b]); without pos_dev, 0 <= pos and
  * pos + n <= S_max are checked. Needs head_dim == 128 and H a multiple of Hkv; qkv and
@@ -338,10 +340,14 @@ OBN_API size_t obn_attention_q8_workspace_bytes(int B, int n, int H, int Hkv, in
  * (device, [B]) is not NULL: seq_len is then their bound (S_max if nothing better is known;
  * the closer the bound, the better the split). Its query t attends to keys
  * [0, L - n + t]; a query without keys (an empty sequence, left padding) gives a zero row.
- * q and the softmax weights enter the products with 22 bits or more, sums are exact integers
- * or f32: results are near those of f32 arithmetic on the cache's values. Scores have to be
- * finite in f32. Needs head_dim == 128, H a multiple of Hkv, 0 <= seq_len <= S_max and a finite
- * scale >= 0; q and out 16-byte, workspace 256-byte aligned, not used by other work in flight. */
+ * The bits that enter the products count against the largest of a row: q has 22 or more against
+ * the row's largest |q| (or 2^-90, if that is larger), the weights times their value scales 22
+ * or more against the row's largest such product. Sums are exact integers or f32, exponentials
+ * f32 (2 ulp): results are near those of f32 arithmetic on the cache's values, and a weight
+ * below 2^-120 of its row's largest may count as zero. Scores, and a row's largest |q| times the
+ * largest |k|, have to be finite in f32. Needs head_dim == 128, H a multiple of Hkv, 0 <=
+ * seq_len <= S_max and a finite scale >= 0; q and out 16-byte, workspace 256-byte aligned, not
+ * used by other work in flight. */
 OBN_API int obn_attention_q8(const float* q, const void* k_cache, const void* v_cache,
                              const float* k_scale, const float* v_scale, int B, int n, int H,
                              int Hkv, int head_dim, int S_max, int seq_len,
@@ -376,9 +382,10 @@ typedef struct obn_logit_rules {
 
 /* out[r, v] = the logits [rows, vocab] under the rules, in the order above: repetition,
  * frequency and presence, biases, mask; a changed value is computed in f64 and rounded once,
- * the others pass unchanged. out may be logits itself (no other overlap). token (nullable, [rows]) takes each
- * row's greedy choice: the largest out[r, v], the lowest v among equals, NaN never; -1 when
- * nothing is above -inf. A single occurrence gives the bits of the sampler's own penalty. */
+ * the others pass unchanged. out may be logits itself (no other overlap). token (nullable,
+ * [rows]) takes each row's greedy choice: the largest out[r, v], the lowest v among equals, NaN
+ * never; -1 when nothing is above -inf. A single occurrence gives the bits of the sampler's own
+ * penalty. */
 OBN_API int obn_logits_process(const float* logits, int rows, int vocab,
                                const obn_logit_rules* rules, float* out, int32_t* token,
                                void* stream);
