@@ -17,11 +17,11 @@
 //    there to the B operand of the second product by two shuffles a 16-key block. K needs no
 //    rearrangement (dims may be contracted in any order), V comes transposed from shared memory
 //    (ldmatrix on 16 x 16 bytes; a byte transpose in registers took 36 against 34 us for 8 x 4 tokens).
-//  * The s32 sums are carried along the keys and only turned into f32 (and rescaled) when
-//    the reference M has to grow, when a weight times its value scale comes above its reference
-//    Vr, or after 2^15 keys (255 * 128 * 2^15 < 2^31). M is set 3 to 4 above the maximum and
-//    Vr to 32 times the largest product: the largest keeps 26 bits or more, and few later keys
-//    exceed them. A value scale alone does not set Vr: a block of large values with small
+//  The s32 sums are carried along the keys and only turned into f32 (and rescaled) when the
+//    reference M has to grow (Vr is then set anew), when a weight times its value scale comes above
+//    its reference Vr, or after 2^15 keys (255 * 128 * 2^15 < 2^31). M is set 3 to 4 above the
+//    maximum and Vr to 32 times the largest product: the largest keeps 26 bits or more, and few
+//    later keys exceed them. A value scale alone does not set Vr: a block of large values with small
 //    weights would take bits from the others.
 //  * Exponentials are ex2.approx (2 ulp, flushed below 2^-126), one for each score: expf's
 //    reduction and its handling of subnormals would be as many instructions again, and the error
@@ -32,10 +32,10 @@
 //    memory. MT consumer warps share a slice when there are more than 4 query rows.
 //
 // 64 sequences of up to 4095 keys, 20/5 heads (176 MB): 43 us with the join, 4.0 TB/s, of which
-// about 8 us are starts and the join; the stream itself runs at 5 TB/s. One sequence of 131072
-// (168 MB): 40 us, 4.2 TB/s. 8 sequences of up to 5000 with 32 rows (24 MB): 33 us, where the
-// products bound the warps: 16 rows cost 1.6 times what 8 do, and half of V's products cost 8 us. 12 warps an SM (3 CTAs whose first warp
-// requests the units between its own) took 51, 42 and 37 us.
+// about 8 us are starts and the join; the stream itself runs at 5 TB/s. One sequence of 131072 (168
+// MB): 40 us, 4.2 TB/s. 8 sequences of up to 5000 with 32 rows (24 MB): 33 us, where the products
+// bound the warps: 16 rows cost 1.6 times what 8 do, and half of V's products cost 8 us. 12 warps
+// an SM (3 CTAs whose first warp requests the units between its own) took 51, 42 and 37 us.
 #include "kvq8.h"
 
 #include <algorithm>
@@ -408,8 +408,10 @@ __global__ __launch_bounds__(32 * (MT * KW + 1), CTAS) void k_attn_q8_few(
 #pragma unroll
         for (int d = 4; d <= 16; d <<= 1) top = fmaxf(top, shx(top, d));
         // only of the rows that need it: no row's bits depend on another's
+        // Vr goes by this slice also when M has grown, as the products before it have shrunk: a large
+        // value of small score at the front must not take the later keys' bits. 1 / Vr stays finite.
         if (mn != M || top > Vr || since >= kFlushSlices)
-          flush(mn, top > Vr ? fmaxf(32.0f * top, FLT_MIN) : Vr);  // 1 / Vr stays finite
+          flush(mn, mn != M || top > Vr ? fmaxf(32.0f * top, FLT_MIN) : Vr);
       }
       uint32_t b[2][2];  // weights: [digits 0 1 / 2 3][block]
 #pragma unroll

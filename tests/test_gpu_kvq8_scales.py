@@ -123,6 +123,23 @@ def test_one_far_scale(n, H, Hkv, exp):
                     np.full(-(-S // ref.BLOCK), 2.0 ** exp), B)
 
 
+@pytest.mark.parametrize("n,H,Hkv", ROWS)
+@pytest.mark.parametrize("S,B", [(150, 1), (700, 1), (700, 80), (3000, 1)])
+@pytest.mark.parametrize("exp,rise", [(12, 20), (30, 40), (100, 120), (0, 100), (-20, 60)])
+def test_large_values_before_larger_scores(n, H, Hkv, S, B, exp, rise):
+    """The first block's values are 2^exp times the others', and the scores grow by `rise` binary
+    digits along the keys: what was large against the first scores takes no bits from the rest."""
+    torch = need_cuda()
+    rng = np.random.default_rng(S + n + rise)
+    nb = -(-S // ref.BLOCK)
+    vs = np.exp2(rng.integers(-3, 4, nb).astype(np.float64))
+    vs[0] *= 2.0 ** exp
+    vs[nb // 2] = 0.0
+    log2w = np.linspace(0, rise, S).astype(np.int64) + rng.integers(-2, 3, S)
+    log2w[nb // 2 * ref.BLOCK:nb // 2 * ref.BLOCK + ref.BLOCK] += 7  # the weightiest have no values
+    run_planted(torch, rng, n, H, Hkv, log2w, vs, B)
+
+
 def any_scales(torch, rng, B, S, Hkv, k_exp, v_exp):
     """A cache whose scales are any numbers, no powers of two; its f64 values and value scales."""
     att = importlib.import_module("0xbitnet_b200.attention")
