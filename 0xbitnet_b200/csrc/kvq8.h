@@ -51,23 +51,6 @@ cudaError_t launch_attention_q8_many(const float* q, const Q8Cache& c, int n, in
                                      const int* lens_dev, float scale_log2, float* out, void* ws,
                                      cudaStream_t s);
 
-// Launch with programmatic dependent launch allowed.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
-
 // Raises a kernel's dynamic shared memory limit on the current device, once for each.
 template <auto kKernel>
 cudaError_t allow_smem(size_t bytes) {

@@ -17,7 +17,7 @@
 //    there to the B operand of the second product by two shuffles a 16-key block. K needs no
 //    rearrangement (dims may be contracted in any order), V comes transposed from shared memory
 //    (ldmatrix on 16 x 16 bytes; a byte transpose in registers took 36 against 34 us for 8 x 4 tokens).
-//  The s32 sums are carried along the keys and only turned into f32 (and rescaled) when the
+//  * The s32 sums are carried along the keys and only turned into f32 (and rescaled) when the
 //    reference M has to grow (Vr is then set anew), when a weight times its value scale comes above
 //    its reference Vr, or after 2^15 keys (255 * 128 * 2^15 < 2^31). M is set 3 to 4 above the
 //    maximum and Vr to 32 times the largest product: the largest keeps 26 bits or more, and few

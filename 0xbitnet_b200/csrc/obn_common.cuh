@@ -137,6 +137,23 @@ OBN_DEVINL void pdl_launch_dependents() {
 // Blocks until every prerequisite grid has completed and its writes are visible.
 OBN_DEVINL void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Launch with programmatic dependent launch allowed.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                       Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 // ---- integer dot product ------------------------------------------------------
 // acc + sum_{b<4} a.byte[b] * b.byte[b], a unsigned codes, b signed int8.
 OBN_DEVINL int dp4a_us(uint32_t a, uint32_t b, int c) {
