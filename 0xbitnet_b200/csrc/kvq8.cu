@@ -46,8 +46,10 @@ OBN_DEVINL float exp_scale(int e) {  // 2^e for a normal exponent
 // its group; a warp takes one row of one head (a lane four dims) at a time.
 //  * Angles are p * base^(-2i/128) in turns, reduced in f64 (an f32 angle is off by 6e-3 at
 //    position 1e5); their sines and cosines, about 50 f64 operations each, are shared by
-//    the CTA's heads. k is rotated in f64, so that a code is off only where f64 is; q in f32;
-//    v times a power of two is exact in f32.
+//    the CTA's heads. k is rotated in f64, so that a code is off only where f64 is. q is
+//    rotated in f32 with rounded sines and cosines (3.7e-8 from the exact one, rounded once 2.5e-8):
+//    it is f32 in any case, attention holds it in 22 bits or more, and f64 would rotate four times
+//    as many rows of q as of k. v times a power of two is exact in f32.
 //  * A block's scale has to be known before its first code: the raw k and v rows stay in
 //    registers (kKeep per warp) from one pass over memory.
 // 2048 tokens of 20 + 2 x 5 heads (31 MB in, 24 MB out): 17.4 us from cold caches, 3.2 TB/s; it
