@@ -177,10 +177,9 @@ class BitNetDecoder:
                     B, 1, H, d, ctx))), dtype=torch.uint8, device=dev)
             else:
                 self.attn_ws = att.attention_q8_workspace(self.caches[0], H, 1)
-                # positions with the last step's token, 0 for a sequence without one; and
-                # whether that step's positions were on the device
+                # positions with the last step's token, 0 (or less) for a sequence without
+                # one; kept on the device alone, where replayed steps write it
                 self.lengths = torch.ones((B,), dtype=torch.int32, device=dev)
-                self._ragged = False
             self.logits = torch.empty((B, cfg.vocab), **f32)
             self.lm_ws = torch.empty(max(1, int(lib().obn_lm_head_workspace_bytes(B, D))),
                                      dtype=torch.uint8, device=dev)
@@ -215,12 +214,9 @@ class BitNetDecoder:
                 raise TypeError("positions per sequence need the 8-bit cache (kv_bits=8)")
             return pos + 1
         if not ragged:
-            if self._ragged:
-                self.lengths.fill_(1)
-            self._ragged = False
+            self.lengths.fill_(1)
             return pos + 1
         att._check(pos, "pos", torch.int32, self.lengths.get_device(), self.B)
-        self._ragged = True
         torch.add(pos.view(-1), 1, out=self.lengths)
         return self.lengths.masked_fill_(self.lengths > self.ctx, 0)
 
@@ -268,7 +264,7 @@ class BitNetDecoder:
         greedy token (-1: nothing allowed, or no token in the step) in self.ids for the
         next step."""
         logits_process(logits, rules, out=logits, token=self.ids)
-        if self.kv_bits == 8 and self._ragged:
+        if self.kv_bits == 8:
             self.ids.masked_fill_(self.lengths <= 0, -1)
         return self.ids
 

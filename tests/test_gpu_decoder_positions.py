@@ -108,3 +108,28 @@ def test_refused_positions_change_nothing():
         assert np.array_equal(a, b)
     assert min(tokens(torch, m, [[3], [4]], [1, 2])) >= 0  # any shape of B elements
     m.close()
+
+
+def test_replayed_steps_between_steps_for_all():
+    """A captured step with positions on the device and eager ones with a position for all, in
+    turn, each followed by an eager pick: what was called last counts."""
+    torch = need_cuda()
+    m, ctx = decoder(2, 20, seed=3), 20
+    pos = torch.tensor([4, ctx], dtype=torch.int32, device="cuda")
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        m.ids.copy_(torch.tensor([1, 2], dtype=torch.int32))
+        m.step(pos)
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = m.step(pos)
+        for _ in range(2):
+            assert min(m.pick(m.step(5), no_rules()).cpu().tolist()) >= 0
+            m.ids.copy_(torch.tensor([1, 2], dtype=torch.int32))
+            g.replay()
+            got = m.pick(out, no_rules()).cpu().tolist()
+            assert got[0] >= 0 and got[1] == -1
+            m.ids.copy_(torch.tensor([1, 2], dtype=torch.int32))
+        del g
+    m.close()
